@@ -311,6 +311,60 @@ int vk_attend_chunk(const vk_attn_geom* g, const void* q, const void* K, const v
                     const int* tile_count, int n_tiles, int nv_cap, const void* proj, int ldp, void* part, int nsplit, void* out,
                     int R, vk_stream_t stream);
 
+/* ---- Rotary positions and the paged append as operators of their own; attention over a shared prefix. The model's own
+ * layers rotate inside vk_attn_prep (volundr.py:663-664; batch.py:224-259); these serve callers with other layouts, head sizes
+ * and scalings. dtype: 0 bf16, 1 fp16. Strides are in elements; the elements of a head lie side by side. */
+/* out[r, h, :] = x[r, h, :] with its first `dims` elements (even, <= D <= 1024) turned by pos[r] * freq[i] (freq: fp64
+ * [dims / 2]) and multiplied by magnitude: pairs (i, i + dims / 2), or (2i, 2i + 1) when interleaved. inverse: the transposed
+ * rotation. out may be x with the same strides; no other overlap. */
+int vk_rope(int dtype, const void* x, long long x_row, long long x_head, void* out, long long out_row, long long out_head,
+            const int* pos, const double* freq, int dims, int interleaved, int inverse, float magnitude, int rows, int heads,
+            int D, vk_stream_t stream);
+/* Row r's keys (rotated by pos[r]) and values go to token slot[r] (slot null: pos[r]) of sequence seq[r] (null: r): page
+ * table[seq, slot / 64], row slot % 64 of K, V [n_pages, KVH, 64, D]. q (optional, with q_out): rotated alongside. A negative
+ * slot is padding: nothing of the row is written. Rows of a call name different places. A page outside the pool, a sequence
+ * or a slot outside the table: status word, K and V of the row skipped. */
+typedef struct vk_append_args {
+    int dtype, rows, Hq, KVH, D, dims, interleaved;
+    float magnitude;
+    const void *q, *k, *v;
+    long long q_row, q_head, k_row, k_head, v_row, v_head;
+    void* q_out;
+    long long qo_row, qo_head;
+    void *K, *V;
+    const int *table, *pos, *slot, *seq;
+    const double* freq;
+    int n_seqs, max_pages, n_pages;
+} vk_append_args;
+int vk_kv_append(const vk_append_args* a, vk_stream_t stream);
+/* Decode attention of sequences that share a prompt prefix: row r = b * T + t (the T newest tokens of sequence b) attends
+ * the first *prefix_len tokens of the pages prefix_pages[max_prefix_pages] and the first lens[r] tokens of its sequence's
+ * pages table[b, max_pages]; out = softmax(scale q k) v, times sigmoid(gate) when gate is given. D 64 or 128; every pointer
+ * 16-byte aligned, strides multiples of 8. lens[r] < 0: a padded row, its output is left as it was; no visible key:
+ * zeros. Lengths beyond the page lists are clamped, pages outside the pool replaced by page 0, both reported in the status
+ * word. At most 65536 rows and 2^31 - 1 key rows (n_pages * KVH * 64) in the pool, else -3. The per-sequence form is
+ * vk_attend_decode. workspace: scratch of the call, needs no initial value; calls that overlap on the GPU need one each. */
+typedef struct vk_prefix_args {
+    int dtype, seqs, T, Hq, KVH, D;
+    float scale;
+    const void* q;
+    long long q_row, q_head;
+    const void* gate;
+    long long gate_row, gate_head;
+    void* out;
+    long long out_row, out_head;
+    const void *K, *V;
+    int n_pages;
+    const int* prefix_pages;
+    int max_prefix_pages;
+    const int* prefix_len;
+    const int* table;
+    int max_pages;
+    const int* lens;
+} vk_prefix_args;
+size_t vk_attend_prefix_workspace_bytes(const vk_prefix_args* a);
+int vk_attend_prefix(const vk_prefix_args* a, void* workspace, size_t workspace_bytes, vk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

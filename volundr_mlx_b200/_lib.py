@@ -3,7 +3,7 @@
 There is no CPU or PyTorch fallback behind these calls: a missing library or a non-zero return raises."""
 import ctypes
 import os
-from ctypes import c_int, c_size_t, c_void_p, c_char_p, c_float, c_double
+from ctypes import c_int, c_longlong, c_size_t, c_void_p, c_char_p, c_float, c_double
 from pathlib import Path
 
 _LIB = None
@@ -82,8 +82,34 @@ SIGNATURES = {
     "vk_attend_scratch_bytes": (c_size_t, [c_void_p, c_int, c_int]),
     "vk_attend_chunk_smem_bytes": (c_size_t, [c_void_p, c_int]),
     "vk_attend_chunk": (c_int, [c_void_p] * 12 + [c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    "vk_rope": (c_int, [c_int, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_int,
+                        c_int, c_int, c_float, c_int, c_int, c_int, c_void_p]),
+    "vk_kv_append": (c_int, [c_void_p, c_void_p]),
+    "vk_attend_prefix_workspace_bytes": (c_size_t, [c_void_p]),
+    "vk_attend_prefix": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "vk_attend_decode": (c_int, [c_void_p] * 11 + [c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
 }
+
+
+class AppendArgs(ctypes.Structure):
+    """vk_append_args of include/volundr_b200.h."""
+    _fields_ = ([(n, c_int) for n in ("dtype", "rows", "Hq", "KVH", "D", "dims", "interleaved")] + [("magnitude", c_float)]
+                + [(n, c_void_p) for n in ("q", "k", "v")]
+                + [(n, c_longlong) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+                + [("q_out", c_void_p), ("qo_row", c_longlong), ("qo_head", c_longlong)]
+                + [(n, c_void_p) for n in ("K", "V", "table", "pos", "slot", "seq", "freq")]
+                + [(n, c_int) for n in ("n_seqs", "max_pages", "n_pages")])
+
+
+class PrefixArgs(ctypes.Structure):
+    """vk_prefix_args of include/volundr_b200.h."""
+    _fields_ = ([(n, c_int) for n in ("dtype", "seqs", "T", "Hq", "KVH", "D")] + [("scale", c_float)]
+                + [("q", c_void_p), ("q_row", c_longlong), ("q_head", c_longlong),
+                   ("gate", c_void_p), ("gate_row", c_longlong), ("gate_head", c_longlong),
+                   ("out", c_void_p), ("out_row", c_longlong), ("out_head", c_longlong),
+                   ("K", c_void_p), ("V", c_void_p), ("n_pages", c_int), ("prefix_pages", c_void_p),
+                   ("max_prefix_pages", c_int), ("prefix_len", c_void_p), ("table", c_void_p), ("max_pages", c_int),
+                   ("lens", c_void_p)])
 
 
 def path() -> Path:

@@ -11,6 +11,10 @@
 #define VK_ENOSPC (-2)
 #define VK_ETOOBIG (-3)  // the problem exceeds a fixed capacity of the entry point
 
+// Storage types of the operators that take more than bf16 (their `dtype` argument).
+#define VK_BF16 0
+#define VK_FP16 1
+
 // Device-side status word: 0 = fine; otherwise the code of the first kernel that gave up on a bounded wait or met
 // an out-of-range index. Read (and cleared) by vk_status_read at the caller's sync point.
 __device__ int g_vk_status = 0;  // (the library is one translation unit: volundr_b200.cu)
