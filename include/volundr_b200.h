@@ -317,9 +317,17 @@ int vk_attend_chunk(const vk_attn_geom* g, const void* q, const void* K, const v
 /* out[r, h, :] = x[r, h, :] with its first `dims` elements (even, <= D <= 1024) turned by pos[r] * freq[i] (freq: fp64
  * [dims / 2]) and multiplied by magnitude: pairs (i, i + dims / 2), or (2i, 2i + 1) when interleaved. inverse: the transposed
  * rotation. out may be x with the same strides; no other overlap. */
-int vk_rope(int dtype, const void* x, long long x_row, long long x_head, void* out, long long out_row, long long out_head,
-            const int* pos, const double* freq, int dims, int interleaved, int inverse, float magnitude, int rows, int heads,
-            int D, vk_stream_t stream);
+typedef struct vk_rope_args {
+    int dtype, rows, heads, D, dims, interleaved, inverse;
+    float magnitude;
+    const void* x;
+    long long x_row, x_head;
+    void* out;
+    long long out_row, out_head;
+    const int* pos;
+    const double* freq;
+} vk_rope_args;
+int vk_rope(const vk_rope_args* a, vk_stream_t stream);
 /* Row r's keys (rotated by pos[r]) and values go to token slot[r] (slot null: pos[r]) of sequence seq[r] (null: r): page
  * table[seq, slot / 64], row slot % 64 of K, V [n_pages, KVH, 64, D]. q (optional, with q_out): rotated alongside. A negative
  * slot is padding: nothing of the row is written. Rows of a call name different places. A page outside the pool, a sequence

@@ -48,19 +48,22 @@ A = 0x10000   # an address that no refused call may touch
 
 
 def rope_args(**kw):
-    d = dict(dtype=0, x=A, x_row=128, x_head=64, out=A, out_row=128, out_head=64, pos=A, freq=A, dims=64, inter=0, inverse=0,
-             magnitude=1.0, rows=4, heads=2, D=64)
+    a = _lib.RopeArgs()
+    d = dict(dtype=0, rows=4, heads=2, D=64, dims=64, interleaved=0, inverse=0, magnitude=1.0, x=A, x_row=128, x_head=64, out=A, out_row=128,
+             out_head=64, pos=A, freq=A)
     d.update(kw)
-    return list(d.values())
+    for k, v in d.items():
+        setattr(a, k, v)
+    return a
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=2), dict(dtype=-1), dict(dims=3), dict(dims=66), dict(dims=-2), dict(D=0), dict(D=1026, dims=2),
                                  dict(rows=-1), dict(heads=0), dict(x=None), dict(out=None), dict(pos=None), dict(freq=None), dict(x=A + 1),
                                  dict(out_row=10), dict(out_head=10), dict(x_row=-1), dict(x_head=-1), dict(magnitude=math.nan)])
 def test_rope_refuses(L, bad):
-    assert L.vk_rope(*rope_args(**bad), None) == -1
-    if "rows" not in bad:
-        assert L.vk_rope(*rope_args(rows=0), None) == 0
+    assert L.vk_rope(ctypes.byref(rope_args(**bad)), None) == -1
+    assert L.vk_rope(ctypes.byref(rope_args(rows=0)), None) == 0
+    assert L.vk_rope(None, None) == -1
 
 
 def append_args(**kw):

@@ -3,6 +3,7 @@
 There is no CPU or PyTorch fallback behind these calls: a missing library or a non-zero return raises."""
 import ctypes
 import os
+import struct
 from ctypes import c_int, c_longlong, c_size_t, c_void_p, c_char_p, c_float, c_double
 from pathlib import Path
 
@@ -82,13 +83,19 @@ SIGNATURES = {
     "vk_attend_scratch_bytes": (c_size_t, [c_void_p, c_int, c_int]),
     "vk_attend_chunk_smem_bytes": (c_size_t, [c_void_p, c_int]),
     "vk_attend_chunk": (c_int, [c_void_p] * 12 + [c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p]),
-    "vk_rope": (c_int, [c_int, c_void_p, c_longlong, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_int,
-                        c_int, c_int, c_float, c_int, c_int, c_int, c_void_p]),
+    "vk_rope": (c_int, [c_void_p, c_void_p]),
     "vk_kv_append": (c_int, [c_void_p, c_void_p]),
     "vk_attend_prefix_workspace_bytes": (c_size_t, [c_void_p]),
     "vk_attend_prefix": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "vk_attend_decode": (c_int, [c_void_p] * 11 + [c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
 }
+
+
+class RopeArgs(ctypes.Structure):
+    """vk_rope_args of include/volundr_b200.h."""
+    _fields_ = ([(n, c_int) for n in ("dtype", "rows", "heads", "D", "dims", "interleaved", "inverse")] + [("magnitude", c_float)]
+                + [("x", c_void_p), ("x_row", c_longlong), ("x_head", c_longlong),
+                   ("out", c_void_p), ("out_row", c_longlong), ("out_head", c_longlong), ("pos", c_void_p), ("freq", c_void_p)])
 
 
 class AppendArgs(ctypes.Structure):
@@ -110,6 +117,17 @@ class PrefixArgs(ctypes.Structure):
                    ("K", c_void_p), ("V", c_void_p), ("n_pages", c_int), ("prefix_pages", c_void_p),
                    ("max_prefix_pages", c_int), ("prefix_len", c_void_p), ("table", c_void_p), ("max_pages", c_int),
                    ("lens", c_void_p)])
+
+
+def _pack(cls):
+    """pack(*fields) -> the bytes of a struct of class cls: one call instead of an attribute store per field."""
+    s = struct.Struct("@" + "".join({c_int: "i", c_float: "f", c_void_p: "P", c_longlong: "q"}[t] for _, t in cls._fields_)
+                      + "0P")     # (padded at the end as the C struct is)
+    assert s.size == ctypes.sizeof(cls)
+    return s.pack
+
+
+ROPE_PACK, APPEND_PACK, PREFIX_PACK = _pack(RopeArgs), _pack(AppendArgs), _pack(PrefixArgs)
 
 
 def path() -> Path:

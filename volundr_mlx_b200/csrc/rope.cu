@@ -171,6 +171,17 @@ int rope_ysplit(int rows, int items) {
 
 extern "C" {
 
+struct vk_rope_args {
+    int dtype, rows, heads, D, dims, interleaved, inverse;
+    float magnitude;
+    const void* x;
+    long long x_row, x_head;
+    void* out;
+    long long out_row, out_head;
+    const int* pos;
+    const double* freq;
+};
+
 struct vk_append_args {
     int dtype, rows, Hq, KVH, D, dims, interleaved;
     float magnitude;
@@ -184,24 +195,22 @@ struct vk_append_args {
     int n_seqs, max_pages, n_pages;
 };
 
-int vk_rope(int dtype, const void* x, long long x_row, long long x_head, void* out, long long out_row, long long out_head,
-            const int* pos, const double* freq, int dims, int interleaved, int inverse, float magnitude, int rows, int heads,
-            int D, cudaStream_t stream) {
-    if (!rope_shape_ok(dtype, rows, D, dims, freq, magnitude) || heads <= 0 || heads > 65536) return VK_EINVAL;
-    if (x_row < 0 || x_head < 0 || (rows > 1 && out_row < D) || (heads > 1 && out_head < D)) return VK_EINVAL;
-    if (rows == 0) return VK_OK;
-    if (x == nullptr || out == nullptr || pos == nullptr) return VK_EINVAL;
-    if (((uintptr_t)x | (uintptr_t)out) & 1) return VK_EINVAL;
+int vk_rope(const vk_rope_args* a, cudaStream_t stream) {
+    if (a == nullptr || !rope_shape_ok(a->dtype, a->rows, a->D, a->dims, a->freq, a->magnitude) || a->heads <= 0 || a->heads > 65536) return VK_EINVAL;
+    if (a->x_row < 0 || a->x_head < 0 || (a->rows > 1 && a->out_row < a->D) || (a->heads > 1 && a->out_head < a->D)) return VK_EINVAL;
+    if (a->rows == 0) return VK_OK;
+    if (a->x == nullptr || a->out == nullptr || a->pos == nullptr) return VK_EINVAL;
+    if (((uintptr_t)a->x | (uintptr_t)a->out) & 1) return VK_EINVAL;
     RopeParams p = {};
-    p.s[0] = RopeRows{x, out, x_row, x_head, out_row, out_head, heads, 1};
-    p.pos = pos; p.freq = freq; p.D = D; p.dims = dims; p.interleaved = interleaved != 0; p.inverse = inverse != 0;
-    p.magnitude = magnitude; p.heads = heads;
+    p.s[0] = RopeRows{a->x, a->out, a->x_row, a->x_head, a->out_row, a->out_head, a->heads, 1};
+    p.pos = a->pos; p.freq = a->freq; p.D = a->D; p.dims = a->dims; p.interleaved = a->interleaved != 0; p.inverse = a->inverse != 0;
+    p.magnitude = a->magnitude; p.heads = a->heads;
     PieceRule r;
-    r.rows(x, x_row, x_head);
-    r.rows(out, out_row, out_head);
-    const int vec = r.vec(D, dims, interleaved);
-    const int ys = rope_ysplit(rows, heads * ((D + vec - 1) / vec));
-    return (int)(dtype == VK_BF16 ? rope_launch<__nv_bfloat16>(vec, p, rows, ys, stream) : rope_launch<__half>(vec, p, rows, ys, stream));
+    r.rows(a->x, a->x_row, a->x_head);
+    r.rows(a->out, a->out_row, a->out_head);
+    const int vec = r.vec(a->D, a->dims, a->interleaved);
+    const int ys = rope_ysplit(a->rows, a->heads * ((a->D + vec - 1) / vec));
+    return (int)(a->dtype == VK_BF16 ? rope_launch<__nv_bfloat16>(vec, p, a->rows, ys, stream) : rope_launch<__half>(vec, p, a->rows, ys, stream));
 }
 
 int vk_kv_append(const vk_append_args* a, cudaStream_t stream) {

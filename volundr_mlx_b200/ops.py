@@ -1,6 +1,4 @@
 """torch-facing wrappers of the C ABI: tensors in, tensors out, raw pointers and the current stream underneath."""
-import ctypes
-
 import torch
 
 from . import _lib
@@ -158,64 +156,85 @@ def check_status(device=None):
 
 
 # ---------------------------------------------------------------- rotary positions, paged append, shared-prefix attention
+# (These run once per layer and step beside kernels of a few microseconds: every check is one or two attribute reads, and the
+# arguments go down as one packed struct.)
 PAGE = 64
 _TYPES = {BF16: 0, torch.float16: 1}
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the stream of torch.cuda.current_stream(index), as an integer
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _refuse(what):
+    raise ValueError(what)
 
 
-def _same(dev, **tensors):
-    """Every given tensor lives on the CUDA device `dev` and carries no gradient these operators would lose."""
-    _need(dev.type == "cuda", "CUDA tensors are required: there is no CPU path")
-    for name, t in tensors.items():
-        if t is not None:
-            _need(t.device == dev, f"{name} is on {t.device}, not on {dev}")
-            _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient: the operator records none")
+def _on(idx, t, name, floating=False):
+    """t lives on CUDA device idx and carries no gradient that the operator would lose."""
+    if idx < 0:
+        _refuse("CUDA tensors are required: there is no CPU path")
+    if t.get_device() != idx:
+        _refuse(f"{name} is on {t.device}, not on cuda:{idx}")
+    if floating and t.requires_grad and torch.is_grad_enabled():
+        _refuse(f"{name} requires a gradient: the operator records none")
 
 
-def _heads(name, t, dtype, rows=None, heads=None, D=None):
-    """[rows, heads, D] of a 16-bit type, elements of a head side by side; rows and heads may be strided."""
-    _need(t.dim() == 3 and t.dtype == dtype, f"{name}: a [rows, heads, D] tensor of {dtype}")
-    _need(all(w is None or n == w for n, w in zip(t.shape, (rows, heads, D))), f"{name}: shape {tuple(t.shape)}")
-    _need(t.shape[2] <= 1 or t.stride(2) == 1, f"{name}: the elements of a head must lie side by side")
+def _heads(idx, t, name, dtype, rows=None, heads=None, D=None):
+    """[rows, heads, D] of `dtype`, the elements of a head side by side, rows and heads strided: its shape and strides."""
+    _on(idx, t, name, True)
+    sh, st = t.shape, t.stride()
+    if t.dtype != dtype or len(sh) != 3:
+        _refuse(f"{name}: a [rows, heads, D] tensor of {dtype}")
+    if (D is not None and sh[2] != D) or (rows is not None and sh[0] != rows) or (heads is not None and sh[1] != heads):
+        _refuse(f"{name}: shape {tuple(sh)}")
+    if st[2] != 1 and sh[2] > 1:
+        _refuse(f"{name}: the elements of a head must lie side by side")
+    return sh, st
 
 
-def _ints(name, t, *shape):
-    _need(t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape, f"{name}: contiguous int32 {shape}")
+def _ints(idx, t, name, *shape):
+    _on(idx, t, name)
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.shape != shape:
+        _refuse(f"{name}: contiguous int32 {shape}")
 
 
-def _pool(K, V, dtype):
-    for name, t in (("K", K), ("V", V)):
-        _need(t.dim() == 4 and t.dtype == dtype and t.is_contiguous() and t.shape == K.shape and t.shape[2] == PAGE,
-              f"{name}: contiguous pages [n_pages, kv heads, {PAGE}, D] of {dtype}")
+def _table(idx, t, name):
+    _on(idx, t, name)
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 2:
+        _refuse(f"{name}: contiguous int32 [sequences, pages]")
+    return t.shape
 
 
-def _turns(freq, D, dev):
+def _pools(idx, K, V, dtype):
+    """K, V: contiguous pages [n_pages, kv heads, PAGE, D]; their shape."""
+    _on(idx, K, "K", True)
+    _on(idx, V, "V", True)
+    sh = K.shape
+    if len(sh) != 4 or sh[2] != PAGE or sh != V.shape or K.dtype != dtype or V.dtype != dtype or sh[0] == 0 or sh[1] == 0:
+        _refuse(f"K, V: pages [n_pages, kv heads, {PAGE}, D] of {dtype}")
+    if not (K.is_contiguous() and V.is_contiguous()):
+        _refuse("K, V: contiguous pages")
+    return sh
+
+
+def _turned(idx, freq, D):
+    """Rotated elements of a head."""
     if freq is None:
         return 0
-    _same(dev, freq=freq)
-    _need(freq.dtype == torch.float64 and freq.dim() == 1 and freq.is_contiguous(), "freq: contiguous float64 [dims / 2]")
-    _need(2 * freq.numel() <= D, f"freq: {2 * freq.numel()} rotated elements in a head of {D}")
-    return 2 * freq.numel()
+    _on(idx, freq, "freq", True)
+    n = 2 * freq.numel()
+    if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous() or n > D:
+        _refuse(f"freq: contiguous float64 [dims / 2], dims at most the head's {D} elements")
+    return n
 
 
-class _On:
-    """The launch's device made current (only when it is not), so that the stream and the launch belong to the tensors."""
-
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return _stream()
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _launch(idx, fn, what, *args):
+    """fn(*args, stream) on the current stream of device idx, that device current."""
+    if idx == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, _raw_stream(idx))
+    if rc:
+        _lib.check(rc, what)
 
 
 def rope(x, pos, freq, *, interleaved=False, magnitude=1.0, inverse=False, out=None):
@@ -225,22 +244,21 @@ def rope(x, pos, freq, *, interleaved=False, magnitude=1.0, inverse=False, out=N
     contexts). inverse: the transposed rotation, which is also the gradient of the plain one. out may be x itself (same
     strides); any other overlap with x is the caller's error. The model's own layers rotate inside vk_attn_prep
     (volundr.py:663-664)."""
-    _same(x.device, pos=pos, x=x, out=out)
-    _need(x.dtype in _TYPES, "x: bfloat16 or float16")
-    _heads("x", x, x.dtype)
-    rows, heads, D = x.shape
-    _ints("pos", pos, rows)
-    dims = _turns(freq, D, x.device)
+    idx, dtype = x.get_device(), x.dtype
+    if dtype not in _TYPES:
+        _refuse("x: bfloat16 or float16")
+    (rows, heads, D), xs = _heads(idx, x, "x", dtype)
+    _ints(idx, pos, "pos", rows)
+    dims = _turned(idx, freq, D)
     if out is None:
-        out = torch.empty((rows, heads, D), dtype=x.dtype, device=x.device)
-    _heads("out", out, x.dtype, rows, heads, D)
-    _need(out.data_ptr() != x.data_ptr() or out.stride() == x.stride(), "out overlaps x with other strides")
-    if rows == 0 or heads == 0:
-        return out
-    with _On(x.device) as st:
-        _lib.check(_lib.lib().vk_rope(_TYPES[x.dtype], _p(x), x.stride(0), x.stride(1), _p(out), out.stride(0), out.stride(1),
-                                      _p(pos), _p(freq), dims, int(interleaved), int(inverse), float(magnitude), rows, heads, D,
-                                      st), "vk_rope")
+        out = torch.empty((rows, heads, D), dtype=dtype, device=x.device)
+    os = _heads(idx, out, "out", dtype, rows, heads, D)[1]
+    if os != xs and out.data_ptr() == x.data_ptr():
+        _refuse("out overlaps x with other strides")
+    if rows and heads:
+        _launch(idx, _lib.lib().vk_rope, "vk_rope",
+                _lib.ROPE_PACK(_TYPES[dtype], rows, heads, D, dims, bool(interleaved), bool(inverse), magnitude, x.data_ptr(), xs[0],
+                               xs[1], out.data_ptr(), os[0], os[1], pos.data_ptr(), 0 if freq is None else freq.data_ptr()))
     return out
 
 
@@ -251,40 +269,43 @@ def kv_append(k, v, K, V, table, pos, freq=None, *, slot=None, seq=None, q=None,
     is padding: nothing of it is written. Rows of one call must name different (seq, slot) places: two rows on one place
     leave a mixture of both. A page outside the pool, or a slot beyond the table, is reported by check_status and
     skipped. slot and pos differ where a sequence's first tokens are a prefix held elsewhere (attend_prefix)."""
-    dev = k.device
-    _same(dev, k=k, v=v, K=K, V=V, table=table, pos=pos, slot=slot, seq=seq, q=q, q_out=q_out)
-    _need(k.dtype in _TYPES, "k: bfloat16 or float16")
-    _heads("k", k, k.dtype)
-    rows, KVH, D = k.shape
-    _heads("v", v, k.dtype, rows, KVH, D)
-    _pool(K, V, k.dtype)
-    _need(K.shape[0] > 0 and K.shape[1] == KVH and K.shape[3] == D, "K, V: kv heads and head size of k")
-    _need(table.dim() == 2 and table.numel() > 0, "table: [sequences, pages]")
-    _ints("table", table, *table.shape)
-    for name, t in (("pos", pos), ("slot", slot), ("seq", seq)):
-        if t is not None:
-            _ints(name, t, rows)
-    _need(seq is not None or rows <= table.shape[0], "more rows than sequences: give seq")
-    a = _lib.AppendArgs()
-    a.dims = _turns(freq, D, dev)
+    idx, dtype = k.get_device(), k.dtype
+    if dtype not in _TYPES:
+        _refuse("k: bfloat16 or float16")
+    (rows, KVH, D), ks = _heads(idx, k, "k", dtype)
+    vs = _heads(idx, v, "v", dtype, rows, KVH, D)[1]
+    pages = _pools(idx, K, V, dtype)
+    if pages[1] != KVH or pages[3] != D:
+        _refuse("K, V: kv heads and head size of k")
+    seqs, max_pages = _table(idx, table, "table")
+    _ints(idx, pos, "pos", rows)
+    if slot is not None:
+        _ints(idx, slot, "slot", rows)
+    if seq is not None:
+        _ints(idx, seq, "seq", rows)
+    elif rows > seqs:
+        _refuse("more rows than sequences: give seq")
+    dims = _turned(idx, freq, D)
+    H, qp, qs, op, os = 0, 0, (0, 0), 0, (0, 0)
     if q is not None:
-        _heads("q", q, k.dtype, rows, None, D)
+        qsh, qs = _heads(idx, q, "q", dtype, rows, None, D)
+        H, qp = qsh[1], q.data_ptr()
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        _heads("q_out", q_out, k.dtype, *q.shape)
-        _need(q_out.data_ptr() != q.data_ptr() or q_out.stride() == q.stride(), "q_out overlaps q with other strides")
-        a.Hq, a.q, a.q_row, a.q_head = q.shape[1], _p(q), q.stride(0), q.stride(1)
-        a.q_out, a.qo_row, a.qo_head = _p(q_out), q_out.stride(0), q_out.stride(1)
-    else:
-        _need(q_out is None, "q_out without q")
-    if rows == 0:
-        return q_out
-    a.dtype, a.rows, a.KVH, a.D, a.interleaved, a.magnitude = _TYPES[k.dtype], rows, KVH, D, int(interleaved), float(magnitude)
-    a.k, a.v, a.k_row, a.k_head, a.v_row, a.v_head = _p(k), _p(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1)
-    a.K, a.V, a.table, a.pos, a.slot, a.seq, a.freq = _p(K), _p(V), _p(table), _p(pos), _p(slot), _p(seq), _p(freq)
-    a.n_seqs, a.max_pages, a.n_pages = table.shape[0], table.shape[1], K.shape[0]
-    with _On(dev) as st:
-        _lib.check(_lib.lib().vk_kv_append(ctypes.byref(a), st), "vk_kv_append")
+            q_out = torch.empty(qsh, dtype=dtype, device=q.device)
+        os, op = _heads(idx, q_out, "q_out", dtype, rows, H, D)[1], q_out.data_ptr()
+        if os != qs and op == qp:
+            _refuse("q_out overlaps q with other strides")
+    elif q_out is not None:
+        _refuse("q_out without q")
+    if rows:
+        if not (seqs and max_pages):
+            _refuse("table: at least one sequence and one page")
+        _launch(idx, _lib.lib().vk_kv_append, "vk_kv_append",
+                _lib.APPEND_PACK(_TYPES[dtype], rows, H, KVH, D, dims, bool(interleaved), magnitude, qp, k.data_ptr(), v.data_ptr(),
+                                 qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], op, os[0], os[1], K.data_ptr(), V.data_ptr(),
+                                 table.data_ptr(), pos.data_ptr(), 0 if slot is None else slot.data_ptr(),
+                                 0 if seq is None else seq.data_ptr(), 0 if freq is None else freq.data_ptr(), seqs, max_pages,
+                                 pages[0]))
     return q_out
 
 
@@ -298,44 +319,40 @@ def attend_prefix(q, K, V, prefix_pages, prefix_len, table, lens, *, T=1, scale=
     Keys and values behind a sequence's last visible token may hold anything; those that one of a sequence's T rows sees
     must be finite for all of its rows. Sums and statistics are fp32, probabilities meet the values in the
     storage type. The per-sequence form without a shared part is vk_attend_decode."""
-    dev = q.device
-    _same(dev, q=q, K=K, V=V, prefix_pages=prefix_pages, prefix_len=prefix_len, table=table, lens=lens, gate=gate, out=out)
-    _need(q.dtype in _TYPES, "q: bfloat16 or float16")
-    _heads("q", q, q.dtype)
-    R, H, D = q.shape
-    _pool(K, V, q.dtype)
-    KVH = K.shape[1]
-    _need(D in (64, 128) and K.shape[3] == D, "head size: 64 or 128, the same in q and the pages")
-    _need(K.shape[0] > 0 and KVH > 0 and H > 0 and H % KVH == 0, "query heads: a multiple of the pages' kv heads")
-    _need(T >= 1 and R % T == 0 and table.dim() == 2 and table.shape[0] == R // T, "table: one row per T rows of q")
-    _ints("table", table, *table.shape)
-    _ints("lens", lens, R)
-    _ints("prefix_len", prefix_len, 1)
-    _need(prefix_pages.dim() == 1, "prefix_pages: [n]")
-    _ints("prefix_pages", prefix_pages, *prefix_pages.shape)
+    idx, dtype = q.get_device(), q.dtype
+    if dtype not in _TYPES:
+        _refuse("q: bfloat16 or float16")
+    (R, H, D), qs = _heads(idx, q, "q", dtype)
+    n_pages, KVH, _, PD = _pools(idx, K, V, dtype)
+    if PD != D or D not in (64, 128):
+        _refuse("head size: 64 or 128, the same in q and the pages")
+    if H == 0 or H % KVH:
+        _refuse("query heads: a multiple of the pages' kv heads")
+    seqs, max_pages = _table(idx, table, "table")
+    if T < 1 or seqs * T != R:
+        _refuse("table: one row per T rows of q")
+    _ints(idx, lens, "lens", R)
+    _ints(idx, prefix_len, "prefix_len", 1)
+    _ints(idx, prefix_pages, "prefix_pages", prefix_pages.numel())
     if out is None:
-        out = torch.zeros((R, H, D), dtype=q.dtype, device=dev)
-    for name, t in (("q", q), ("gate", gate), ("out", out)):
-        if t is not None:
-            _heads(name, t, q.dtype, R, H, D)
-            _need(t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0, f"{name}: 16-byte aligned heads")
-    scale = D ** -0.5 if scale is None else float(scale)
-    _need(0.0 < scale < float("inf"), "scale: positive and finite")
-    if R == 0:
-        return out
-    a = _lib.PrefixArgs()
-    a.dtype, a.seqs, a.T, a.Hq, a.KVH, a.D, a.scale = _TYPES[q.dtype], R // T, T, H, KVH, D, scale
-    a.q, a.q_row, a.q_head = _p(q), q.stride(0), q.stride(1)
+        out = torch.zeros((R, H, D), dtype=dtype, device=q.device)
+    os = _heads(idx, out, "out", dtype, R, H, D)[1]
+    gp, gs = 0, (0, 0)
     if gate is not None:
-        a.gate, a.gate_row, a.gate_head = _p(gate), gate.stride(0), gate.stride(1)
-    a.out, a.out_row, a.out_head = _p(out), out.stride(0), out.stride(1)
-    a.K, a.V, a.n_pages = _p(K), _p(V), K.shape[0]
-    a.prefix_pages, a.max_prefix_pages, a.prefix_len = _p(prefix_pages), prefix_pages.numel(), _p(prefix_len)
-    a.table, a.max_pages, a.lens = _p(table), table.shape[1], _p(lens)
-    L = _lib.lib()
-    with _On(dev) as st:
+        gs, gp = _heads(idx, gate, "gate", dtype, R, H, D)[1], gate.data_ptr()
+    qp, op = q.data_ptr(), out.data_ptr()
+    if (qp | op | gp) & 15 or (qs[0] | qs[1] | os[0] | os[1] | gs[0] | gs[1]) & 7:
+        _refuse("q, out, gate: 16-byte aligned heads")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        _refuse("scale: positive and finite")
+    if R:
+        L = _lib.lib()
+        a = _lib.PREFIX_PACK(_TYPES[dtype], seqs, T, H, KVH, D, scale, qp, qs[0], qs[1], gp, gs[0], gs[1], op, os[0], os[1],
+                             K.data_ptr(), V.data_ptr(), n_pages, prefix_pages.data_ptr(), prefix_pages.numel(),
+                             prefix_len.data_ptr(), table.data_ptr(), max_pages, lens.data_ptr())
         # scratch of its own per call, from the caching allocator: calls on other streams or in other graphs share nothing
-        need = L.vk_attend_prefix_workspace_bytes(ctypes.byref(a))
-        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        _lib.check(L.vk_attend_prefix(ctypes.byref(a), _p(ws), ws.numel(), st), "vk_attend_prefix")
+        need = L.vk_attend_prefix_workspace_bytes(a)
+        ws = torch.empty(need or 16, dtype=torch.uint8, device=q.device)
+        _launch(idx, L.vk_attend_prefix, "vk_attend_prefix", a, ws.data_ptr(), need)
     return out
