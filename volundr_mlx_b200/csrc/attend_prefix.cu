@@ -28,17 +28,23 @@ extern "C" struct vk_prefix_args {
 
 namespace {
 
-// A unit of work is 128 keys of one kv head against a tile of up to 128 (row, query head) pairs, one tensor-memory lane each:
-//   S[128 x 128] = Q K^T (tcgen05.mma, Q and K in shared memory), P = exp2(S - m) in registers, O[128 x D] += P V with P in
-//   tensor memory (over S) and V in shared memory.
+// A unit of work is 128 keys of one kv head against a tile of (row, query head) pairs. Two forms:
+//   wide   up to 128 pairs, one tensor-memory lane each: S[128 x 128] = Q K^T (tcgen05.mma, Q and K in shared memory),
+//          P = exp2(S - m) in registers, O[128 x D] += P V with P in tensor memory (over S) and V in shared memory. Two
+//          streams (softmax warpgroups) take turns on the tensor core: two tiles on the same keys, or one tile's even and odd units;
+//   narrow up to 64 pairs (a sequence's own keys, a small batch): mma.sync m16n8k16, the unit's keys dealt to the eight warps
+//          in chunks of 16, each warp with its own running maximum, sum and output, joined when the job ends. No round
+//          trips between warps and tensor core, and a 16-row tile does not pay for 128.
 // A job is a run of units: a tile, or two tiles that share the keys, against the prefix or against one sequence's own keys.
-// All jobs' units lie on one line, weighted by their tiles, and every CTA takes an equal interval of it.
-constexpr int kPfTile = 128, kPfKeys = 128;
-// warps 0-3 and 4-7: softmax of two streams; 8: copies; 9: tensor core; 10, 11 fill the third warpgroup, whose registers go to
-// the softmax (a row of S is 128 registers): 168 a thread at launch, then 216 + 216 + 72 = 3 x 168
+// All jobs lie on one line, each as long as it is expected to take, and every CTA takes an equal interval of it.
+constexpr int kPfTile = 128, kPfKeys = 128, kPfNarrow = 64;
+// warps 0-3 and 4-7: softmax of two streams (narrow: eight equals); 8: copies; 9: tensor core; 10, 11 fill the third
+// warpgroup, whose registers go to the softmax (a row of S is 128 registers): 168 a thread at launch, then 216 + 216 + 72 = 3 x 168
 constexpr int kPfThreads = 384;
 constexpr int kPfSoftmaxRegs = 216, kPfOtherRegs = 72;
-constexpr int kPfWindow = 64;            // sequences whose unit counts are kept in shared memory
+constexpr int kPfWindow = 64;            // sequences whose key counts are kept in shared memory
+// Lengths on the line of work: a job's fixed part, a unit of one tile, of two tiles, of the narrow form
+struct PfCost { int fixed, one, two; };
 
 template <int D> struct PfCfg {
     static constexpr int kTileBytes = 128 * D * 2;
@@ -50,24 +56,41 @@ struct PfParams {
     CUtensorMap mapK, mapV;
     vk_prefix_args a;
     int G, MT, ST;             // query heads per kv head; tiles of the prefix part, of a sequence's own part
+    int narrowP, narrowO;      // the form of either part
+    PfCost costP, costO;
     int rowsP, rowsO;          // rows of a slot (a slot holds one job's partial result of one CTA)
-    long long *head, *cum;     // workspace: {total, CTAs, prefix length}; exclusive sums of the sequences' unit counts
+    int *head, *cum;           // workspace: {total, CTAs, prefix length, end of the prefix jobs}; where a sequence's jobs begin
     float2 *mlP, *mlO;         // running maximum (log2 units) and sum
     float *oP, *oO;            // unnormalised output
 };
 
 struct PfJob {
-    int own, h, b, grp, u0, u1, tiles;
-    long long slot;
+    int own, h, b, grp, u0, u1, tiles, narrow, slot;
 };
 
-__device__ __forceinline__ long long pf_low(long long c, long long total, int n) { return c * total / n; }
-
-// The part of a job [A, A + w * units) that lies in [lo, hi): units [u0, u1)
-__device__ __forceinline__ void pf_units(long long A, int w, long long lo, long long hi, int& u0, int& u1) {
-    u0 = (int)((lo - A + w - 1) / w);
-    u1 = (int)((hi - A + w - 1) / w);
+// CTA c's interval of the line: equal shares, the first total % n one longer
+__device__ __forceinline__ int pf_low(int c, int total, int n) { return c * (total / n) + min(c, total % n); }
+__device__ __forceinline__ int pf_cta_of(int x, int total, int n) {
+    const int q = total / n, r = total % n, edge = r * (q + 1);
+    return x < edge ? x / (q + 1) : r + (x - edge) / q;
 }
+
+// Units of a job that begin (behind its fixed part) inside [lo, hi), both relative to the job's start
+__device__ __forceinline__ void pf_units(int fixed, int w, int nu, int lo, int hi, int& u0, int& u1) {
+    u0 = lo <= fixed ? 0 : min(nu, (lo - fixed + w - 1) / w);
+    u1 = hi <= fixed ? 0 : min(nu, (hi - fixed + w - 1) / w);
+}
+
+// Where the jobs of one kv head lie: tile groups one after another, all of two tiles but perhaps the last
+struct PfHead {
+    int groups, len2, len, nu;     // tile groups; length of a group of two; of all groups
+    __device__ __forceinline__ PfHead(int tiles, int nu_, const PfCost& c) {
+        groups = (tiles + 1) / 2;
+        nu = nu_;
+        len2 = c.fixed + c.two * nu;
+        len = nu == 0 ? 0 : (tiles / 2) * len2 + (tiles & 1) * (c.fixed + c.one * nu);
+    }
+};
 
 __device__ __forceinline__ int pf_clamp(int n, int pages) {
     const int cap = pages * 64;
@@ -78,72 +101,58 @@ __device__ __forceinline__ int pf_clamp(int n, int pages) {
 // Keys of sequence b's own pages that any of its rows sees
 __device__ __forceinline__ int pf_own_keys(const vk_prefix_args& a, int b) {
     int n = 0;
-    for (int t = 0; t < a.T; t++) n = max(n, a.lens[(long long)b * a.T + t]);
+    for (int t = 0; t < a.T; t++) n = max(n, a.lens[b * a.T + t]);
     return pf_clamp(n, a.max_pages);
 }
 __device__ __forceinline__ int pf_nu(int keys) { return (keys + kPfKeys - 1) / kPfKeys; }
 
 struct PfShared {
     uint64_t full[10], empty[10], qfull[2], sready[2], pready[2], odone[2], join[2];
-    long long total, lo, hi, cb0;
-    int b0, P, n, fail;
+    int total, lo, hi, cb0, b0, P, n, fail;
     uint32_t tmem;
+    int red[kPfThreads / 32];
     int keys[kPfWindow];
-    long long red[kPfThreads / 32];
+    float2 ml[8][16];
 };
 
 struct PfIter {
-    long long cur, hi, cb;
-    int b, keys;
-    int npu;
-    long long perHead, prefixCost;
+    int cur, hi, cb, b, keys, prefixEnd;
     __device__ void init(const PfParams& p, const PfShared& s) {
-        npu = pf_nu(s.P);
-        perHead = (long long)npu * p.MT;
-        prefixCost = perHead * p.a.KVH;
+        prefixEnd = PfHead(p.MT, pf_nu(s.P), p.costP).len * p.a.KVH;
         cur = s.lo; hi = s.hi;
         b = s.b0; cb = s.cb0;
         keys = b < p.a.seqs ? s.keys[0] : 0;
     }
-    __device__ int own_keys(const PfParams& p, const PfShared& s, int i) const {
-        return i - s.b0 < kPfWindow ? s.keys[i - s.b0] : pf_own_keys(p.a, i);
-    }
     __device__ bool next(const PfParams& p, const PfShared& s, PfJob& j) {
         while (cur < hi) {
-            long long A, B;
-            int w;
-            if (cur < prefixCost) {
+            int A, tiles;
+            if (cur < prefixEnd) {
                 j.own = 0; j.b = 0;
-                j.h = (int)(cur / perHead);
-                j.grp = (int)((cur - j.h * perHead) / (2 * npu));
-                w = 2 * j.grp + 1 < p.MT ? 2 : 1;
-                A = j.h * perHead + (long long)j.grp * 2 * npu;
-                B = A + (long long)w * npu;
-                j.slot = (long long)j.h * ((p.MT + 1) / 2) + j.grp;
+                tiles = p.MT;
+                A = 0;
             } else {
-                long long cost;
-                int nu;
                 for (;;) {
-                    nu = pf_nu(keys);
-                    cost = (long long)nu * p.a.KVH * p.ST;
-                    if (cur < cb + cost) break;
-                    cb += cost;
+                    const int len = PfHead(p.ST, pf_nu(keys), p.costO).len * p.a.KVH;
+                    if (cur < cb + len) break;
+                    cb += len;
                     b++;
-                    keys = own_keys(p, s, b);
+                    keys = b - s.b0 < kPfWindow ? s.keys[b - s.b0] : pf_own_keys(p.a, b);
                 }
-                const long long rel = cur - cb, per = (long long)nu * p.ST;
                 j.own = 1; j.b = b;
-                j.h = (int)(rel / per);
-                j.grp = (int)((rel - j.h * per) / (2 * nu));
-                w = 2 * j.grp + 1 < p.ST ? 2 : 1;
-                A = cb + j.h * per + (long long)j.grp * 2 * nu;
-                B = A + (long long)w * nu;
-                j.slot = ((long long)b * p.a.KVH + j.h) * ((p.ST + 1) / 2) + j.grp;
+                tiles = p.ST;
+                A = cb;
             }
-            const long long e = hi < B ? hi : B;
-            pf_units(A, w, cur, e, j.u0, j.u1);
-            j.tiles = w;
-            j.slot += blockIdx.x;
+            const PfCost& c = j.own ? p.costO : p.costP;
+            const PfHead hd(tiles, pf_nu(j.own ? keys : s.P), c);
+            j.h = (cur - A) / hd.len;
+            A += j.h * hd.len;
+            j.grp = (cur - A) / hd.len2;
+            A += j.grp * hd.len2;
+            j.tiles = 2 * j.grp + 1 < tiles ? 2 : 1;
+            j.narrow = j.own ? p.narrowO : p.narrowP;
+            const int w = j.tiles == 2 ? c.two : c.one, e = min(hi, A + c.fixed + w * hd.nu);
+            pf_units(c.fixed, w, hd.nu, cur - A, e - A, j.u0, j.u1);
+            j.slot = (j.b * p.a.KVH + j.h) * hd.groups + j.grp + blockIdx.x;
             cur = e;
             if (j.u1 > j.u0) return true;
         }
@@ -151,17 +160,58 @@ struct PfIter {
     }
 };
 
-// Order of a job's copies in the stage ring: as the tensor core uses them (two score products ahead of the values).
-__device__ __forceinline__ int pf_stage_k(int i, int tiles) { return tiles == 2 ? 2 * i : (i == 0 ? 0 : 2 * i - 1); }
-__device__ __forceinline__ int pf_stage_v(int i, int n, int tiles) { return tiles == 2 ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2); }
+// Order of a job's copies in the stage ring. pairs: K and V of one unit after another (two tiles; narrow jobs); else the tensor
+// core runs two score products ahead of the values.
+__device__ __forceinline__ int pf_stage_k(int i, bool pairs) { return pairs ? 2 * i : (i == 0 ? 0 : 2 * i - 1); }
+__device__ __forceinline__ int pf_stage_v(int i, int n, bool pairs) { return pairs ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2); }
 
 __device__ __forceinline__ void pf_mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // A bounded wait of a whole warp, with one answer for all its lanes
 __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase)); }
+// (whole-warp calls, one elected lane acts: the operands stay warp-uniform)
 __device__ __forceinline__ void pf_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
+}
+// A stage's "empty" barrier counts the eight warps of the narrow form: seven arrivals now, the eighth when the MMAs are done
+__device__ __forceinline__ void pf_commit_stage(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e mbarrier.arrive.shared::cta.b64 _, [%0], 7;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(ta), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void pf_ldm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void pf_ldm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <typename T> __device__ __forceinline__ void pf_mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void pf_tma(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -208,6 +258,151 @@ __device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// A narrow job: the eight warps (16-row tile warp % wm of the pairs, keys of chunks warp / wm, + 8 / wm, ... of every unit).
+template <typename T, int D>
+__device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const PfJob& j, int keys, uint8_t* smem, const uint8_t* ring, int base,
+                                          uint32_t nj) {
+    constexpr int NST = PfCfg<D>::kStages, TB = PfCfg<D>::kTileBytes;
+    const vk_prefix_args& a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rows = (j.own ? a.T : a.seqs * a.T) * p.G;
+    const int wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4, ng = 8 / wm;
+    const int mt = warp % wm, kg = warp / wm;
+    const bool work = mt * 16 < rows;
+    const float sl2 = a.scale * 1.4426950408889634f;
+    // Q as A fragments: rows g and g + 8 of the tile
+    uint32_t qa[D / 16][4];
+    int see[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int m = mt * 16 + g + 8 * i, r = (j.own ? j.b * a.T : 0) + m / p.G;
+        const bool live = m < rows;
+        const T* q = (const T*)a.q + (live ? r * a.q_row + (j.h * p.G + m % p.G) * a.q_head : 0);
+        see[i] = !live ? 0 : j.own ? min(keys, max(0, a.lens[r])) : keys;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+            qa[k][i] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 2 * t) : 0u;
+            qa[k][2 + i] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + 2 * t) : 0u;
+        }
+    }
+    float o[D / 8][4], ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    bool ok = true;
+    for (int u = j.u0; u < j.u1; u++) {
+        const int ck = base + 2 * (u - j.u0), cv = ck + 1, sk = ck % NST, sv = cv % NST;
+        const uint32_t kb = smem_u32(ring + (size_t)sk * TB), vb = smem_u32(ring + (size_t)sv * TB);
+        const int kv = min(kPfKeys, keys - u * kPfKeys);
+        if (!pf_wait(&s.full[sk], (uint32_t)((ck / NST) & 1)) || !pf_wait(&s.full[sv], (uint32_t)((cv / NST) & 1))) { ok = false; break; }
+        if (work) {
+            for (int c = kg; c * 16 < kv; c += ng) {
+                float x[2][4] = {};
+                const int krow = c * 16 + (lane >> 4) * 8 + (lane & 7);     // K rows as the N side: two tiles of eight keys
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    uint32_t b[4];
+                    const int ch = 2 * k + ((lane >> 3) & 1);
+                    pf_ldm4(b, kb + (ch >> 3) * 16384 + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4));
+                    pf_mma16<T>(x[0], qa[k], b[0], b[1]);
+                    pf_mma16<T>(x[1], qa[k], b[2], b[3]);
+                }
+                const int key0 = u * kPfKeys + c * 16 + 2 * t;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            if (key0 + 8 * n + e >= see[i]) x[n][2 * i + e] = -INFINITY;
+                    float top = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * sl2;
+                    float f = 1.f;
+                    if (top > ref[i] + 8.f || ref[i] == -INFINITY) {        // (as in the wide form)
+                        if (ref[i] != -INFINITY) f = pf_ex2(ref[i] - top);
+                        ref[i] = top;
+                    }
+                    if (__any_sync(0xffffffffu, f != 1.f)) {
+                        l[i] *= f;
+#pragma unroll
+                        for (int n = 0; n < D / 8; n++) { o[n][2 * i] *= f; o[n][2 * i + 1] *= f; }
+                    }
+                    const float off = ref[i] == -INFINITY ? 0.f : ref[i];
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            x[n][2 * i + e] = pf_ex2(fmaf(x[n][2 * i + e], sl2, -off));
+                            l[i] += x[n][2 * i + e];
+                        }
+                }
+                const uint32_t pa[4] = {pf_pack<T>(x[0][0], x[0][1]), pf_pack<T>(x[0][2], x[0][3]), pf_pack<T>(x[1][0], x[1][1]), pf_pack<T>(x[1][2], x[1][3])};
+                if (c * 16 + 16 > kv) {   // values behind the last key may be anything: zeros (0 * NaN is NaN)
+                    const int z0 = kv, zn = (c * 16 + 16 - kv) * (D / 8);
+                    for (int e = lane; e < zn; e += 32) {
+                        const int zr = z0 + e / (D / 8), ch = e % (D / 8);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + (ch >> 3) * 16384 + zr * 128 + ((ch & 7) << 4)), "r"(0u) : "memory");
+                    }
+                    __syncwarp();
+                }
+                const int vrow = c * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);   // V rows as the K side, transposed on the way
+#pragma unroll
+                for (int n = 0; n < D / 16; n++) {
+                    uint32_t b[4];
+                    const int ch = 2 * n + (lane >> 4);
+                    pf_ldm4t(b, vb + (ch >> 3) * 16384 + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4));
+                    pf_mma16<T>(o[2 * n], pa, b[0], b[1]);
+                    pf_mma16<T>(o[2 * n + 1], pa, b[2], b[3]);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) {
+            pf_mbar_arrive(&s.empty[sk]);
+            pf_mbar_arrive(&s.empty[sv]);
+        }
+    }
+    if (!ok) return false;
+    // ---- the warps' parts joined in shared memory (where the wide form keeps Q), written as the job's partial result
+    float* const buf = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        const int row = g + 8 * i;
+        if (t == 0) s.ml[warp][row] = make_float2(ref[i], l[i]);
+#pragma unroll
+        for (int n = 0; n < D / 8; n++)   // (blocks of eight columns swapped by row: the eight rows of a store hit different banks)
+            *reinterpret_cast<float2*>(buf + (warp * 16 + row) * D + ((n ^ (row & 7)) * 8 + 2 * t)) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    }
+    __syncwarp();
+    if (lane == 0) pf_mbar_arrive(&s.join[0]);
+    if (!pf_wait(&s.join[0], nj & 1)) return false;
+    const long long at = (long long)j.slot * (j.own ? p.rowsO : p.rowsP);
+    float2* ml = (j.own ? p.mlO : p.mlP) + at;
+    float* out = (j.own ? p.oO : p.oP) + at * D;
+    for (int e = threadIdx.x; e < rows * (D / 4); e += 256) {
+        const int m = e / (D / 4), col = (e % (D / 4)) * 4, row = m & 15, w0 = m >> 4;
+        float mx = -INFINITY;
+        for (int k = 0; k < ng; k++) mx = fmaxf(mx, s.ml[w0 + k * wm][row].x);
+        const float off = mx == -INFINITY ? 0.f : mx;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+        for (int k = 0; k < ng; k++) {
+            const float2 x = s.ml[w0 + k * wm][row];
+            const float f = pf_ex2(x.x - off);
+            const float4 v = *reinterpret_cast<const float4*>(buf + ((w0 + k * wm) * 16 + row) * D + (((col >> 3) ^ (row & 7)) * 8 + (col & 7)));
+            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+            sum += x.y * f;
+        }
+        *reinterpret_cast<float4*>(out + (long long)m * D + col) = acc;
+        if (col == 0) ml[m] = make_float2(mx, sum);
+    }
+    __syncwarp();
+    if (lane == 0) pf_mbar_arrive(&s.join[1]);
+    return true;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __grid_constant__ PfParams p) {
     using Cfg = PfCfg<D>;
@@ -220,13 +415,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < NST; i++) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 1); }
+        for (int i = 0; i < NST; i++) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 8); }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.qfull[i], 128);
             mbar_init(&s.sready[i], 1);
             mbar_init(&s.pready[i], 128);
             mbar_init(&s.odone[i], 1);
-            mbar_init(&s.join[i], 256);
+            mbar_init(&s.join[i], 8);
         }
         mbar_fence_init();
         s.fail = 0;
@@ -237,61 +432,69 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
     }
     pdl_wait();
     pdl_launch_dependents();
-    // ---- the line of work: total, this CTA's interval, the sequence in which it starts
-    if (tid == 0) s.P = pf_clamp(*a.prefix_len, a.max_prefix_pages);
-    const int chunks = (a.seqs + kPfThreads - 1) / kPfThreads;
-    long long running = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        // (pass 0: the total; pass 1: exclusive sums, in which the interval's start is looked up)
-        if (pass == 1) {
-            if (tid == 0) {
-                const long long total = (long long)pf_nu(s.P) * p.MT * a.KVH + running * a.KVH * p.ST;
-                s.total = total;
-                s.n = (int)(total < gridDim.x ? total : gridDim.x);
-                if (s.n > 0 && blockIdx.x < s.n) {
-                    s.lo = pf_low(blockIdx.x, total, s.n);
-                    s.hi = pf_low(blockIdx.x + 1, total, s.n);
-                } else {
-                    s.lo = s.hi = total;
-                }
-                s.b0 = a.seqs;
-                s.cb0 = total;
-                if (blockIdx.x == 0) { p.head[0] = total; p.head[1] = s.n; p.head[2] = s.P; }
-            }
-            __syncthreads();
-            running = 0;
-        }
-        for (int c = 0; c < chunks; c++) {
+    // ---- the line of work: its length, this CTA's interval of it, the sequence in which that starts
+    {
+        const int chunks = (a.seqs + kPfThreads - 1) / kPfThreads;
+        const int P = tid == 0 ? pf_clamp(*a.prefix_len, a.max_prefix_pages) : 0;
+        if (tid == 0) s.P = P;
+        int keys = 0, before = 0, len = 0;
+        // lengths of the sequences' jobs, summed over the block: `before` in front of this thread's sequence, the chunk's sum returned
+        auto scan = [&](int c) {
             const int b = c * kPfThreads + tid;
-            const int nu = b < a.seqs ? pf_nu(pf_own_keys(a, b)) : 0;
-            long long v = nu;
+            keys = b < a.seqs ? pf_own_keys(a, b) : 0;
+            len = PfHead(p.ST, pf_nu(keys), p.costO).len * a.KVH;
+            int v = len;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, v, o);
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
                 if (lane >= o) v += u;
             }
+            __syncthreads();
             if (lane == 31) s.red[warp] = v;
             __syncthreads();
-            long long before = running, all = 0;
+            before = v - len;
+            int all = 0;
+#pragma unroll
             for (int i = 0; i < kPfThreads / 32; i++) {
                 if (i < warp) before += s.red[i];
                 all += s.red[i];
             }
-            if (pass == 1 && b < a.seqs) {
-                const long long ex = before + v - nu, base = (long long)pf_nu(s.P) * p.MT * a.KVH, per = (long long)a.KVH * p.ST;
-                if (blockIdx.x == 0) p.cum[b] = ex;
-                // the first sequence with work at or behind the interval's start
-                const long long start = s.lo > base ? s.lo : base;
-                if (nu > 0 && base + ex * per <= start && start < base + (ex + nu) * per) {
-                    s.b0 = b;
-                    s.cb0 = base + ex * per;
-                }
+            return all;
+        };
+        int all = 0;
+        for (int c = 0; c < chunks; c++) all += scan(c);
+        const int base = PfHead(p.MT, pf_nu(s.P), p.costP).len * a.KVH, total = base + all;
+        // (no more CTAs than shares of one unit)
+        const int n = min((int)gridDim.x, total / min(p.costP.one, p.costO.one));
+        const bool has = (int)blockIdx.x < n;
+        const int lo = has ? pf_low(blockIdx.x, total, n) : total, hi = has ? pf_low(blockIdx.x + 1, total, n) : total;
+        const int start = max(lo, base);
+        if (tid == 0) {
+            s.lo = lo;
+            s.hi = hi;
+            s.b0 = a.seqs;
+            s.cb0 = total;
+            if (blockIdx.x == 0) { p.head[0] = total; p.head[1] = n; p.head[2] = P; p.head[3] = base; }
+        }
+        __syncthreads();
+        int running = base;
+        for (int c = 0; c < chunks; c++) {
+            const int sum = chunks == 1 ? 0 : scan(c);
+            const int b = c * kPfThreads + tid, at = running + before;
+            if (b < a.seqs) {
+                if (blockIdx.x == 0) p.cum[b] = at;
+                if (len > 0 && at <= start && start < at + len) { s.b0 = b; s.cb0 = at; }
             }
-            running += all;
-            __syncthreads();
+            running += sum;
+        }
+        __syncthreads();
+        const int i = tid - s.b0;      // (one chunk: the thread of a sequence still has its key count)
+        if (chunks == 1) {
+            if (i >= 0 && i < kPfWindow) s.keys[i] = keys;
+        } else if (tid < kPfWindow) {
+            s.keys[tid] = s.b0 + tid < a.seqs ? pf_own_keys(a, s.b0 + tid) : 0;
         }
     }
-    if (tid < kPfWindow) s.keys[tid] = s.b0 + tid < a.seqs ? pf_own_keys(a, s.b0 + tid) : 0;
     pf_fence_before();
     __syncthreads();
     pf_fence_after();
@@ -318,7 +521,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             // copies in the tensor core's order: copy c of the job is K or V of some unit
             for (int c = 0; c < 2 * nu && ok; c++) {
                 int i, isv;
-                if (j.tiles == 2) { i = c >> 1; isv = c & 1; }
+                if (j.tiles == 2 || j.narrow) { i = c >> 1; isv = c & 1; }
                 else if (c == 0) { i = 0; isv = 0; }
                 else if (c == 2 * nu - 1) { i = nu - 1; isv = 1; }
                 else if (c & 1) { i = (c + 1) >> 1; isv = 0; }
@@ -359,8 +562,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             s.fail = 1;
             for (int k = n > NST ? n - NST : 0; k < n; k++) mbar_wait(&s.full[k % NST], (uint32_t)((k / NST) & 1));
         }
-      } else if (warp == 9 && lane == 0) {
-        // ---------------------------------------------------------------- tensor core
+      } else if (warp == 9) {
+        // ---------------------------------------------------------------- tensor core (the wide form)
         {
             constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
             constexpr uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
@@ -370,47 +573,41 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
             while (ok && it.next(p, s, j)) {
                 const int nu = j.u1 - j.u0, steps = nu * j.tiles;
+                if (j.narrow) { base += 2 * nu; continue; }
+                const bool pairs = j.tiles == 2;
                 auto score = [&](int i) {    // S of stream i & 1 = Q K^T of step i
-                    const int sx = i & 1, c = base + pf_stage_k(j.tiles == 2 ? i >> 1 : i, j.tiles), st = c % NST;
-                    if (!mbar_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; return; }
+                    const int sx = i & 1, c = base + pf_stage_k(pairs ? i >> 1 : i, pairs), st = c % NST;
+                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; return; }
                     pf_fence_after();
                     const uint32_t q0 = smem_u32(smem + sx * TB), k0 = smem_u32(ring + (size_t)st * TB);
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++) {
                         const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
                         const uint64_t da = pf_desc(q0 + off, 16), db = pf_desc(k0 + off, 16);
-                        asm volatile(
-                            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem + sx * 128),
-                            "l"(da), "l"(db), "r"(idescS), "r"(kk > 0 ? 1u : 0u)
-                            : "memory");
+                        pf_mma_ss(tmem + sx * 128, da, db, idescS, kk > 0 ? 1u : 0u);
                     }
-                    if (j.tiles == 1 || sx == 1) pf_commit(&s.empty[st]);
+                    if (!pairs || sx == 1) pf_commit_stage(&s.empty[st]);
                     pf_commit(&s.sready[sx]);
                 };
                 for (int x = 0; x < 2 && x < steps && ok; x++) {
-                    if (!mbar_wait(&s.qfull[x], nq[x] & 1)) { ok = false; break; }
+                    if (!pf_wait(&s.qfull[x], nq[x] & 1)) { ok = false; break; }
                     nq[x]++;
                 }
                 if (ok) score(0);
                 if (ok && steps > 1) score(1);
                 for (int i = 0; i < steps && ok; i++) {
-                    const int sx = i & 1, unit = j.tiles == 2 ? i >> 1 : i;
-                    const int c = base + pf_stage_v(unit, nu, j.tiles), st = c % NST;
-                    if (!mbar_wait(&s.full[st], (uint32_t)((c / NST) & 1)) || !mbar_wait(&s.pready[sx], np[sx] & 1)) { ok = false; break; }
+                    const int sx = i & 1, unit = pairs ? i >> 1 : i;
+                    const int c = base + pf_stage_v(unit, nu, pairs), st = c % NST;
+                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1)) || !pf_wait(&s.pready[sx], np[sx] & 1)) { ok = false; break; }
                     np[sx]++;
                     pf_fence_after();
                     const uint32_t v0 = smem_u32(ring + (size_t)st * TB);
 #pragma unroll
                     for (int kk = 0; kk < kPfKeys / 16; kk++) {
                         const uint64_t db = pf_desc(v0 + kk * 2048, 16384);
-                        asm volatile(
-                            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem + 256 + sx * 128),
-                            "r"(tmem + sx * 128 + kk * 8), "l"(db), "r"(idescO), "r"(i >= 2 || kk > 0 ? 1u : 0u)
-                            : "memory");
+                        pf_mma_ts(tmem + 256 + sx * 128, tmem + sx * 128 + kk * 8, db, idescO, i >= 2 || kk > 0 ? 1u : 0u);
                     }
-                    if (j.tiles == 1 || sx == 1) pf_commit(&s.empty[st]);
+                    if (!pairs || sx == 1) pf_commit_stage(&s.empty[st]);
                     if (i + 2 >= steps) pf_commit(&s.odone[sx]);
                     else score(i + 2);
                 }
@@ -431,26 +628,42 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         while (ok && it.next(p, s, j)) {
             const int nu = j.u1 - j.u0, steps = nu * j.tiles;
             const int keys = j.own ? it.keys : P;
+            if (nj > 0 && !pf_wait(&s.join[1], (nj - 1) & 1)) { ok = false; break; }   // the last job's exchange has been read
+            if (j.narrow) {
+                ok = pf_narrow<T, D>(p, s, j, keys, smem, ring, base, nj);
+                nj++;
+                base += 2 * nu;
+                continue;
+            }
             const int mine = (steps + 1 - sx) / 2;                 // steps of this stream
             if (mine == 0) { base += 2 * nu; continue; }           // (one unit of one tile: the other stream alone)
-            // this thread's (row, query head) pair
-            const int tile = j.grp * 2 + (j.tiles == 2 ? sx : 0);
-            const long long m = (long long)tile * 128 + row;
-            const bool live = m < (long long)(j.own ? a.T : a.seqs * a.T) * p.G;
+            // this thread's (row, query head) pair: lane `row` of the tile
+            const int tile0 = (j.grp * 2 + (j.tiles == 2 ? sx : 0)) * 128, m = tile0 + row;
+            const int pairsOf = (j.own ? a.T : a.seqs * a.T) * p.G;
+            const bool live = m < pairsOf;
             int see = 0x7FFFFFFF;                                  // keys it sees (a lane without a pair: zeros, never written)
-            uint8_t* const qdst = smem + sx * TB + row * 128;
             const bool work = __any_sync(0xffffffffu, live);
-            if (live) {
-                const long long r = (j.own ? (long long)j.b * a.T : 0) + m / p.G;
-                const T* q = (const T*)a.q + r * a.q_row + (j.h * p.G + m % p.G) * a.q_head;
+            if (work) {
+                const int r = (j.own ? j.b * a.T : 0) + m / p.G;
+                long long qat = -1;
+                if (live) {
+                    qat = r * a.q_row + (j.h * p.G + m % p.G) * a.q_head;
+                    see = j.own ? min(keys, max(0, a.lens[r])) : P;
+                }
+                // the warp's 32 rows of Q, D / 8 lanes a row, into the operand's swizzled layout
+                constexpr int LPR = D / 8, RPI = 32 / LPR;
+                const int c = lane % LPR;
+                uint4 v[32 / RPI];
 #pragma unroll
-                for (int c = 0; c < D / 8; c++)
-                    *reinterpret_cast<uint4*>(qdst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = reinterpret_cast<const uint4*>(q)[c];
-                see = j.own ? min(keys, max(0, a.lens[r])) : P;
-            } else if (work) {
+                for (int k = 0; k < 32 / RPI; k++) {
+                    const long long at = __shfl_sync(0xffffffffu, qat, k * RPI + lane / LPR);
+                    v[k] = at < 0 ? make_uint4(0u, 0u, 0u, 0u) : reinterpret_cast<const uint4*>((const T*)a.q + at)[c];
+                }
 #pragma unroll
-                for (int c = 0; c < D / 8; c++)
-                    *reinterpret_cast<uint4*>(qdst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+                for (int k = 0; k < 32 / RPI; k++) {
+                    const int qr = (warp & 3) * 32 + k * RPI + lane / LPR;
+                    *reinterpret_cast<uint4*>(smem + sx * TB + (c >> 3) * 16384 + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[k];
+                }
             }
             fence_proxy_async_smem();
             pf_mbar_arrive(&s.qfull[sx]);
@@ -513,7 +726,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 // values behind the last key may be anything, and 0 * NaN is NaN: their rows of the stage become zeros
                 const int kv = keys - key0;
                 if (kv < kPfKeys && (j.tiles == 1 || sx == 0)) {
-                    const int c = base + pf_stage_v(unit, nu, j.tiles), st = c % NST;
+                    const int c = base + pf_stage_v(unit, nu, j.tiles == 2), st = c % NST;
                     if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; break; }
                     uint8_t* v = ring + (size_t)st * TB;
                     for (int e = kv * 8 + row; e < kPfKeys * 8; e += 128)
@@ -532,7 +745,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             pf_fence_after();
             const bool join = j.tiles == 1 && steps > 1;           // both streams hold a part of the same tile
             const int srow = (j.tiles == 2 ? sx * 128 : 0) + row;
-            const long long at = j.slot * (j.own ? p.rowsO : p.rowsP) + srow;
+            const long long at = (long long)j.slot * (j.own ? p.rowsO : p.rowsP) + srow;
             float2* ml = (j.own ? p.mlO : p.mlP) + at;
             float* o = (j.own ? p.oO : p.oP) + at * D;
             if (!join) {
@@ -553,7 +766,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 // the two streams' parts added; each stream's warps write half of the columns
                 // (the pairs are exchanged where the streams' Q lay, which no product reads any more)
                 reinterpret_cast<float2*>(smem + sx * TB)[row] = make_float2(ref, l);
-                pf_mbar_arrive(&s.join[0]);
+                __syncwarp();
+                if (lane == 0) pf_mbar_arrive(&s.join[0]);
                 if (!pf_wait(&s.join[0], nj & 1)) { ok = false; break; }
                 const float2 x0 = reinterpret_cast<const float2*>(smem)[row], x1 = reinterpret_cast<const float2*>(smem + TB)[row];
                 const float mx = fmaxf(x0.x, x1.x), off = mx == -INFINITY ? 0.f : mx;
@@ -576,9 +790,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                     }
                 }
                 pf_fence_before();
-                pf_mbar_arrive(&s.join[1]);
-                if (!pf_wait(&s.join[1], nj & 1)) { ok = false; break; }   // O and the exchanged pairs are free again
-                pf_fence_after();
+                __syncwarp();
+                if (lane == 0) pf_mbar_arrive(&s.join[1]);         // (both streams wait for it before they begin another job)
                 nj++;
             }
         }
@@ -603,43 +816,34 @@ __global__ void __launch_bounds__(128) attend_prefix_merge_kernel(const __grid_c
     const int r = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq, h = hq / p.G, g = hq % p.G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (a.lens[r] < 0) return;
-    const long long total = p.head[0];
-    const int n = (int)p.head[1], npu = pf_nu((int)p.head[2]);
+    const int total = p.head[0], n = p.head[1], P = p.head[2];
     float m = -INFINITY, l = 0.f, o[E] = {};
     for (int own = 0; own < 2; own++) {
-        long long A, slot;
-        int w, nu, srow;
-        if (own) {
-            const int b = r / a.T, mm = (r - b * a.T) * p.G + g, tile = mm / 128, grp = tile / 2;
-            nu = pf_nu(pf_own_keys(a, b));
-            w = 2 * grp + 1 < p.ST ? 2 : 1;
-            A = (long long)npu * p.MT * a.KVH + (p.cum[b] * a.KVH + (long long)h * nu) * p.ST + (long long)grp * 2 * nu;
-            slot = ((long long)b * a.KVH + h) * ((p.ST + 1) / 2) + grp;
-            srow = mm - grp * 256;
-        } else {
-            const long long mm = (long long)r * p.G + g, tile = mm / 128, grp = tile / 2;
-            nu = npu;
-            w = 2 * grp + 1 < p.MT ? 2 : 1;
-            A = ((long long)h * p.MT + grp * 2) * npu;
-            slot = (long long)h * ((p.MT + 1) / 2) + grp;
-            srow = (int)(mm - grp * 256);
-        }
-        if (nu == 0) continue;
-        const long long B = A + (long long)w * nu;
-        const int c0 = (int)(((A + 1) * n - 1) / total), c1 = (int)((B * n - 1) / total);
+        const int b = own ? r / a.T : 0, mm = (own ? r - b * a.T : r) * p.G + g, grp = mm / 256;
+        const PfCost& cost = own ? p.costO : p.costP;
+        const int tiles = own ? p.ST : p.MT;
+        const PfHead hd(tiles, pf_nu(own ? pf_own_keys(a, b) : P), cost);
+        if (hd.nu == 0) continue;
+        const int w = 2 * grp + 1 < tiles ? cost.two : cost.one;
+        const int A = (own ? p.cum[b] : 0) + h * hd.len + grp * hd.len2, B = A + cost.fixed + w * hd.nu;
+        const int slot = (b * a.KVH + h) * hd.groups + grp, srow = mm - grp * 256;
+        const int c0 = pf_cta_of(A, total, n), c1 = pf_cta_of(B - 1, total, n);
+        const long long step = own ? p.rowsO : p.rowsP;
+        const float2* mls = (own ? p.mlO : p.mlP) + slot * step + srow;
+        const float* os = (own ? p.oO : p.oP) + (slot * step + srow) * D + lane;
         for (int c = c0 + warp; c <= c1; c += 4) {
-            const long long lo = pf_low(c, total, n), hi = pf_low(c + 1, total, n);
             int u0, u1;
-            pf_units(A, w, lo > A ? lo : A, hi < B ? hi : B, u0, u1);
+            pf_units(cost.fixed, w, hd.nu, max(pf_low(c, total, n), A) - A, min(pf_low(c + 1, total, n), B) - A, u0, u1);
             if (u1 <= u0) continue;
-            const long long at = (slot + c) * (own ? p.rowsO : p.rowsP) + srow;
-            const float2 x = (own ? p.mlO : p.mlP)[at];
-            const float* src = (own ? p.oO : p.oP) + at * D;
+            const float2 x = mls[c * step];
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = os[c * step * D + e * 32];
             const float mn = fmaxf(m, x.x), off = mn == -INFINITY ? 0.f : mn;
             const float f0 = exp2f(m - off), f1 = exp2f(x.x - off);
             l = l * f0 + x.y * f1;
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] = o[e] * f0 + src[e * 32 + lane] * f1;
+            for (int e = 0; e < E; e++) o[e] = o[e] * f0 + v[e] * f1;
             m = mn;
         }
     }
@@ -706,7 +910,12 @@ int prefix_args_ok(const vk_prefix_args* a) {
     if ((long long)a->n_pages * a->KVH * 64 > 0x7FFFFFFFll || (long long)a->max_prefix_pages * 64 > 0x7FFFFFFFll ||
         (long long)a->max_pages * 64 > 0x7FFFFFFFll)
         return VK_ETOOBIG;
-    if ((long long)a->seqs * a->T > 65536) return VK_ETOOBIG;
+    const long long rows = (long long)a->seqs * a->T;
+    if (rows > 65536 || rows * a->Hq > 0x7FFFFFFFll) return VK_ETOOBIG;
+    // the line of work (at most 16 a unit of two tiles, as much for a job's fixed part) and the slots are 32-bit counts
+    const long long G = a->Hq / a->KVH, gP = (rows * G + 255) / 256, gO = (a->T * G + 255) / 256;
+    if (((long long)a->max_prefix_pages / 2 + 2) * a->KVH * gP * 16 + a->seqs * ((long long)a->max_pages / 2 + 2) * a->KVH * gO * 16 > 0x7FFFFFFFll)
+        return VK_ETOOBIG;
     return VK_OK;
 }
 
@@ -733,6 +942,9 @@ size_t pf_layout(PfParams& p, const vk_prefix_args* a, uint8_t* ws, int ctas) {
     const long long mP = (long long)a->seqs * a->T * p.G, mO = (long long)a->T * p.G;
     p.MT = (int)((mP + 127) / 128);
     p.ST = (int)((mO + 127) / 128);
+    p.narrowP = mP <= kPfNarrow;
+    p.narrowO = mO <= kPfNarrow;
+    p.costP = p.costO = PfCost{4, 4, 8};
     p.rowsP = (int)(mP < 256 ? mP : 256);
     p.rowsO = (int)(mO < 256 ? mO : 256);
     const size_t slotsP = (size_t)a->KVH * ((p.MT + 1) / 2) + ctas, slotsO = (size_t)a->seqs * a->KVH * ((p.ST + 1) / 2) + ctas;
@@ -742,8 +954,8 @@ size_t pf_layout(PfParams& p, const vk_prefix_args* a, uint8_t* ws, int ctas) {
         at += (bytes + 255) & ~(size_t)255;
         return x;
     };
-    p.head = (long long*)take(64);
-    p.cum = (long long*)take((size_t)a->seqs * 8);
+    p.head = (int*)take(64);
+    p.cum = (int*)take((size_t)a->seqs * 4);
     p.mlP = (float2*)take(slotsP * p.rowsP * 8);
     p.mlO = (float2*)take(slotsO * p.rowsO * 8);
     p.oP = (float*)take(slotsP * p.rowsP * a->D * 4);
