@@ -32,17 +32,19 @@ namespace {
 //   wide   up to 128 pairs, one tensor-memory lane each: S[128 x 128] = Q K^T (tcgen05.mma, Q and K in shared memory),
 //          P = exp2(S - m) in registers, O[128 x D] += P V with P in tensor memory (over S) and V in shared memory. Two
 //          streams (softmax warpgroups) take turns on the tensor core: two tiles on the same keys, or one tile's even and odd units;
-//   narrow up to 64 pairs (a sequence's own keys, a small batch): mma.sync m16n8k16, the unit's keys dealt to the eight warps
-//          in chunks of 16, each warp with its own running maximum, sum and output, joined when the job ends. No round
-//          trips between warps and tensor core, and a 16-row tile does not pay for 128.
+//   narrow up to 64 pairs (a sequence's own keys, a small batch): mma.sync m16n8k16 by one warpgroup, the unit's keys dealt to
+//          its warps in chunks of 32, each warp with its own running maximum, sum and output, joined when the job ends.
+//          The two warpgroups take jobs in turn, so that one's start and end lie under the other's units. No round trips
+//          between warps and tensor core, and a 16-row tile does not pay for 128.
 // A job is a run of units: a tile, or two tiles that share the keys, against the prefix or against one sequence's own keys.
 // All jobs lie on one line, each as long as it is expected to take, and every CTA takes an equal interval of it.
 constexpr int kPfTile = 128, kPfKeys = 128, kPfNarrow = 64;
-// warps 0-3 and 4-7: softmax of two streams (narrow: eight equals); 8: copies; 9: tensor core; 10, 11 fill the third
-// warpgroup, whose registers go to the softmax (a row of S is 128 registers): 168 a thread at launch, then 216 + 216 + 72 = 3 x 168
+// warps 0-3 and 4-7: softmax of two streams; 8: copies; 9: tensor core; 10: walks the line of work and hands out the jobs; 11
+// fills the third warpgroup, whose registers go to the softmax (a row of S is 128 registers): 168 a thread at launch, then
+// 216 + 216 + 72 = 3 x 168
 constexpr int kPfThreads = 384;
 constexpr int kPfSoftmaxRegs = 216, kPfOtherRegs = 72;
-constexpr int kPfWindow = 64;            // sequences whose key counts are kept in shared memory
+constexpr int kPfJobs = 4;               // jobs handed out ahead
 // Lengths on the line of work: a job's fixed part, a unit of one tile, of two tiles, of the narrow form
 struct PfCost { int fixed, one, two; };
 
@@ -65,7 +67,12 @@ struct PfParams {
 };
 
 struct PfJob {
-    int own, h, b, grp, u0, u1, tiles, narrow, slot;
+    int kind;                  // -1: no more; bit 0: own pages; bit 1: two tiles; bit 2: narrow
+    int h, b, grp, u0, u1, slot, keys;
+    __device__ __forceinline__ bool own() const { return kind & 1; }
+    __device__ __forceinline__ int tiles() const { return kind & 2 ? 2 : 1; }
+    __device__ __forceinline__ bool narrow() const { return kind & 4; }
+    __device__ __forceinline__ bool pairs() const { return kind & 6; }     // order of the job's copies (below)
 };
 
 // CTA c's interval of the line: equal shares, the first total % n one longer
@@ -107,55 +114,62 @@ __device__ __forceinline__ int pf_own_keys(const vk_prefix_args& a, int b) {
 __device__ __forceinline__ int pf_nu(int keys) { return (keys + kPfKeys - 1) / kPfKeys; }
 
 struct PfShared {
-    uint64_t full[10], empty[10], qfull[2], sready[2], pready[2], odone[2], join[2];
-    int total, lo, hi, cb0, b0, P, n, fail;
+    uint64_t full[10], empty[10], qfull[2], sready[2], pready[2], odone[2], join[2], njoin[2], nturn[2], jfull[kPfJobs], jempty[kPfJobs];
+    PfJob jobs[kPfJobs];
+    int lo, hi, cb0, b0, P, fail;
     uint32_t tmem;
     int red[kPfThreads / 32];
-    int keys[kPfWindow];
     float2 ml[8][16];
 };
 
+// The jobs of [s.lo, s.hi), one after another: walked by a whole warp, lane i holding the key count of sequence window + i
 struct PfIter {
-    int cur, hi, cb, b, keys, prefixEnd;
-    __device__ void init(const PfParams& p, const PfShared& s) {
+    int cur, hi, cb, b, prefixEnd, window, mine, lane;
+    __device__ __forceinline__ void look(const PfParams& p, int from) {
+        window = from;
+        mine = from + lane < p.a.seqs ? pf_own_keys(p.a, from + lane) : 0;
+    }
+    __device__ __forceinline__ void init(const PfParams& p, const PfShared& s, int lane_) {
+        lane = lane_;
         prefixEnd = PfHead(p.MT, pf_nu(s.P), p.costP).len * p.a.KVH;
         cur = s.lo; hi = s.hi;
         b = s.b0; cb = s.cb0;
-        keys = b < p.a.seqs ? s.keys[0] : 0;
+        look(p, b);
     }
-    __device__ bool next(const PfParams& p, const PfShared& s, PfJob& j) {
+    __device__ __forceinline__ bool next(const PfParams& p, const PfShared& s, PfJob& j) {
         while (cur < hi) {
-            int A, tiles;
-            if (cur < prefixEnd) {
-                j.own = 0; j.b = 0;
-                tiles = p.MT;
-                A = 0;
-            } else {
+            int A = 0;
+            const bool own = cur >= prefixEnd;
+            j.b = 0;
+            j.keys = s.P;
+            if (own) {
                 for (;;) {
-                    const int len = PfHead(p.ST, pf_nu(keys), p.costO).len * p.a.KVH;
+                    if (b - window >= 32) look(p, b);
+                    j.keys = __shfl_sync(0xffffffffu, mine, b - window);
+                    const int len = PfHead(p.ST, pf_nu(j.keys), p.costO).len * p.a.KVH;
                     if (cur < cb + len) break;
                     cb += len;
                     b++;
-                    keys = b - s.b0 < kPfWindow ? s.keys[b - s.b0] : pf_own_keys(p.a, b);
                 }
-                j.own = 1; j.b = b;
-                tiles = p.ST;
+                j.b = b;
                 A = cb;
             }
-            const PfCost& c = j.own ? p.costO : p.costP;
-            const PfHead hd(tiles, pf_nu(j.own ? keys : s.P), c);
+            const PfCost& c = own ? p.costO : p.costP;
+            const int tiles = own ? p.ST : p.MT;
+            const PfHead hd(tiles, pf_nu(j.keys), c);
             j.h = (cur - A) / hd.len;
             A += j.h * hd.len;
             j.grp = (cur - A) / hd.len2;
             A += j.grp * hd.len2;
-            j.tiles = 2 * j.grp + 1 < tiles ? 2 : 1;
-            j.narrow = j.own ? p.narrowO : p.narrowP;
-            const int w = j.tiles == 2 ? c.two : c.one, e = min(hi, A + c.fixed + w * hd.nu);
+            const bool two = 2 * j.grp + 1 < tiles;
+            j.kind = (own ? 1 : 0) | (two ? 2 : 0) | ((own ? p.narrowO : p.narrowP) ? 4 : 0);
+            const int w = two ? c.two : c.one, e = min(hi, A + c.fixed + w * hd.nu);
             pf_units(c.fixed, w, hd.nu, cur - A, e - A, j.u0, j.u1);
             j.slot = (j.b * p.a.KVH + j.h) * hd.groups + j.grp + blockIdx.x;
             cur = e;
             if (j.u1 > j.u0) return true;
         }
+        j.kind = -1;
         return false;
     }
 };
@@ -170,6 +184,16 @@ __device__ __forceinline__ void pf_mbar_arrive(uint64_t* bar) {
 }
 // A bounded wait of a whole warp, with one answer for all its lanes
 __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase)); }
+// The next job from the queue (a whole warp; lane 0 hands the place back). False at the end or when a wait ran out (then ok too).
+__device__ __forceinline__ bool pf_next(PfShared& s, PfJob& j, int& nth, bool& ok) {
+    const int q = nth % kPfJobs;
+    if (!ok || !pf_wait(&s.jfull[q], (uint32_t)((nth / kPfJobs) & 1))) { ok = false; return false; }
+    j = s.jobs[q];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) pf_mbar_arrive(&s.jempty[q]);
+    nth++;
+    return j.kind >= 0;
+}
 // (whole-warp calls, one elected lane acts: the operands stay warp-uniform)
 __device__ __forceinline__ void pf_commit(uint64_t* bar) {
     asm volatile(
@@ -177,11 +201,11 @@ __device__ __forceinline__ void pf_commit(uint64_t* bar) {
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
         : "memory");
 }
-// A stage's "empty" barrier counts the eight warps of the narrow form: seven arrivals now, the eighth when the MMAs are done
+// A stage's "empty" barrier counts the four warps of the narrow form: three arrivals now, the fourth when the MMAs are done
 __device__ __forceinline__ void pf_commit_stage(uint64_t* bar) {
     asm volatile(
         "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e mbarrier.arrive.shared::cta.b64 _, [%0], 7;\n\t"
+        "@e mbarrier.arrive.shared::cta.b64 _, [%0], 3;\n\t"
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
         : "memory");
 }
@@ -258,15 +282,18 @@ __device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// A narrow job: the eight warps (16-row tile warp % wm of the pairs, keys of chunks warp / wm, + 8 / wm, ... of every unit).
+// A narrow job, by one warpgroup: 16-row tile warp % wm of the pairs, keys of chunks warp / wm, + 4 / wm, ... of every unit.
+// smem: the warpgroup's own 128 D half-words, where the warps' parts meet; turn: narrow jobs before this one; nn: phases of
+// s.njoin used so far.
 template <typename T, int D>
-__device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const PfJob& j, int keys, uint8_t* smem, const uint8_t* ring, int base,
-                                          uint32_t nj) {
+__device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const PfJob& j, uint8_t* smem, const uint8_t* ring, int base, uint32_t turn,
+                                          uint32_t& nn) {
     constexpr int NST = PfCfg<D>::kStages, TB = PfCfg<D>::kTileBytes;
     const vk_prefix_args& a = p.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rows = (j.own ? a.T : a.seqs * a.T) * p.G;
-    const int wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4, ng = 8 / wm;
+    const int sx = threadIdx.x >> 7, warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const bool own = j.own();
+    const int rows = (own ? a.T : a.seqs * a.T) * p.G, keys = j.keys;
+    const int wm = rows <= 16 ? 1 : rows <= 32 ? 2 : 4, ng = 4 / wm;
     const int mt = warp % wm, kg = warp / wm;
     const bool work = mt * 16 < rows;
     const float sl2 = a.scale * 1.4426950408889634f;
@@ -275,10 +302,10 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
     int see[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const int m = mt * 16 + g + 8 * i, r = (j.own ? j.b * a.T : 0) + m / p.G;
+        const int m = mt * 16 + g + 8 * i, r = (own ? j.b * a.T : 0) + m / p.G;
         const bool live = m < rows;
         const T* q = (const T*)a.q + (live ? r * a.q_row + (j.h * p.G + m % p.G) * a.q_head : 0);
-        see[i] = !live ? 0 : j.own ? min(keys, max(0, a.lens[r])) : keys;
+        see[i] = !live ? 0 : own ? min(keys, max(0, a.lens[r])) : keys;
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
             qa[k][i] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 2 * t) : 0u;
@@ -288,33 +315,44 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
     float o[D / 8][4], ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    bool ok = true;
-    for (int u = j.u0; u < j.u1; u++) {
+    // A stage's barrier tells only its latest two phases apart, so every warp that waits for a copy must know that the one before
+    // it in the same stage has landed: the other warpgroup has seen all of the job before this one.
+    bool ok = turn == 0 || pf_wait(&s.nturn[sx ^ 1], ((turn - 1) >> 1) & 1);
+    for (int u = j.u0; u < j.u1 && ok; u++) {
         const int ck = base + 2 * (u - j.u0), cv = ck + 1, sk = ck % NST, sv = cv % NST;
         const uint32_t kb = smem_u32(ring + (size_t)sk * TB), vb = smem_u32(ring + (size_t)sv * TB);
         const int kv = min(kPfKeys, keys - u * kPfKeys);
         if (!pf_wait(&s.full[sk], (uint32_t)((ck / NST) & 1)) || !pf_wait(&s.full[sv], (uint32_t)((cv / NST) & 1))) { ok = false; break; }
         if (work) {
-            for (int c = kg; c * 16 < kv; c += ng) {
-                float x[2][4] = {};
-                const int krow = c * 16 + (lane >> 4) * 8 + (lane & 7);     // K rows as the N side: two tiles of eight keys
+#pragma unroll 1
+            for (int c = kg; c * 32 < kv; c += ng) {
+                float x[4][4] = {};
+                const int krow = c * 32 + (lane >> 4) * 8 + (lane & 7);     // K rows as the N side: eight keys a tile
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
-                    uint32_t b[4];
                     const int ch = 2 * k + ((lane >> 3) & 1);
-                    pf_ldm4(b, kb + (ch >> 3) * 16384 + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4));
+                    const uint32_t at = kb + (ch >> 3) * 16384 + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4);
+                    uint32_t b[4];
+                    pf_ldm4(b, at);
                     pf_mma16<T>(x[0], qa[k], b[0], b[1]);
                     pf_mma16<T>(x[1], qa[k], b[2], b[3]);
+                    pf_ldm4(b, at + 16 * 128);
+                    pf_mma16<T>(x[2], qa[k], b[0], b[1]);
+                    pf_mma16<T>(x[3], qa[k], b[2], b[3]);
                 }
-                const int key0 = u * kPfKeys + c * 16 + 2 * t;
+                const int key0 = u * kPfKeys + c * 32 + 2 * t;
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
+                    if (__any_sync(0xffffffffu, see[i] < u * kPfKeys + c * 32 + 32)) {
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
+                        for (int n = 0; n < 4; n++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            if (key0 + 8 * n + e >= see[i]) x[n][2 * i + e] = -INFINITY;
-                    float top = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
+                            for (int e = 0; e < 2; e++)
+                                if (key0 + 8 * n + e >= see[i]) x[n][2 * i + e] = -INFINITY;
+                    }
+                    float top = x[0][2 * i];
+#pragma unroll
+                    for (int n = 0; n < 4; n++) top = fmaxf(top, fmaxf(x[n][2 * i], x[n][2 * i + 1]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * sl2;
                     float f = 1.f;
@@ -329,30 +367,34 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
                     }
                     const float off = ref[i] == -INFINITY ? 0.f : ref[i];
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
+                    for (int n = 0; n < 4; n++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             x[n][2 * i + e] = pf_ex2(fmaf(x[n][2 * i + e], sl2, -off));
                             l[i] += x[n][2 * i + e];
                         }
                 }
-                const uint32_t pa[4] = {pf_pack<T>(x[0][0], x[0][1]), pf_pack<T>(x[0][2], x[0][3]), pf_pack<T>(x[1][0], x[1][1]), pf_pack<T>(x[1][2], x[1][3])};
-                if (c * 16 + 16 > kv) {   // values behind the last key may be anything: zeros (0 * NaN is NaN)
-                    const int z0 = kv, zn = (c * 16 + 16 - kv) * (D / 8);
+                if (c * 32 + 32 > kv) {   // values behind the last key may be anything: zeros (0 * NaN is NaN)
+                    const int zn = (c * 32 + 32 - kv) * (D / 8);
                     for (int e = lane; e < zn; e += 32) {
-                        const int zr = z0 + e / (D / 8), ch = e % (D / 8);
+                        const int zr = kv + e / (D / 8), ch = e % (D / 8);
                         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vb + (ch >> 3) * 16384 + zr * 128 + ((ch & 7) << 4)), "r"(0u) : "memory");
                     }
                     __syncwarp();
                 }
-                const int vrow = c * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);   // V rows as the K side, transposed on the way
 #pragma unroll
-                for (int n = 0; n < D / 16; n++) {
-                    uint32_t b[4];
-                    const int ch = 2 * n + (lane >> 4);
-                    pf_ldm4t(b, vb + (ch >> 3) * 16384 + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4));
-                    pf_mma16<T>(o[2 * n], pa, b[0], b[1]);
-                    pf_mma16<T>(o[2 * n + 1], pa, b[2], b[3]);
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t pa[4] = {pf_pack<T>(x[2 * k][0], x[2 * k][1]), pf_pack<T>(x[2 * k][2], x[2 * k][3]),
+                                            pf_pack<T>(x[2 * k + 1][0], x[2 * k + 1][1]), pf_pack<T>(x[2 * k + 1][2], x[2 * k + 1][3])};
+                    const int vrow = c * 32 + k * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);   // V rows as the K side, transposed on the way
+#pragma unroll
+                    for (int n = 0; n < D / 16; n++) {
+                        uint32_t b[4];
+                        const int ch = 2 * n + (lane >> 4);
+                        pf_ldm4t(b, vb + (ch >> 3) * 16384 + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4));
+                        pf_mma16<T>(o[2 * n], pa, b[0], b[1]);
+                        pf_mma16<T>(o[2 * n + 1], pa, b[2], b[3]);
+                    }
                 }
             }
         }
@@ -363,43 +405,70 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
         }
     }
     if (!ok) return false;
-    // ---- the warps' parts joined in shared memory (where the wide form keeps Q), written as the job's partial result
-    float* const buf = reinterpret_cast<float*>(smem);
+    if (lane == 0) pf_mbar_arrive(&s.nturn[sx]);
+    const long long at = (long long)j.slot * (own ? p.rowsO : p.rowsP);
+    float2* ml = (own ? p.mlO : p.mlP) + at;
+    float* out = (own ? p.oO : p.oP) + at * D;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    if (ng == 1) {                       // every warp has all keys of its rows
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int m = mt * 16 + g + 8 * i;
+            if (m < rows) {
+                if (t == 0) ml[m] = make_float2(ref[i], l[i]);
+#pragma unroll
+                for (int n = 0; n < D / 8; n++) *reinterpret_cast<float2*>(out + m * D + n * 8 + 2 * t) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            }
+        }
+        return true;
+    }
+    // ---- the warps' parts joined in shared memory, written as the job's partial result
+    if (nn > 0 && !pf_wait(&s.njoin[sx], (nn - 1) & 1)) return false;      // the last job's have been read
+    float* const buf = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
         const int row = g + 8 * i;
-        if (t == 0) s.ml[warp][row] = make_float2(ref[i], l[i]);
+        if (t == 0) s.ml[sx * 4 + warp][row] = make_float2(ref[i], l[i]);
 #pragma unroll
         for (int n = 0; n < D / 8; n++)   // (blocks of eight columns swapped by row: the eight rows of a store hit different banks)
             *reinterpret_cast<float2*>(buf + (warp * 16 + row) * D + ((n ^ (row & 7)) * 8 + 2 * t)) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
     }
     __syncwarp();
-    if (lane == 0) pf_mbar_arrive(&s.join[0]);
-    if (!pf_wait(&s.join[0], nj & 1)) return false;
-    const long long at = (long long)j.slot * (j.own ? p.rowsO : p.rowsP);
-    float2* ml = (j.own ? p.mlO : p.mlP) + at;
-    float* out = (j.own ? p.oO : p.oP) + at * D;
-    for (int e = threadIdx.x; e < rows * (D / 4); e += 256) {
+    if (lane == 0) pf_mbar_arrive(&s.njoin[sx]);
+    if (!pf_wait(&s.njoin[sx], nn & 1)) return false;
+    for (int e = threadIdx.x & 127; e < rows * (D / 4); e += 128) {
         const int m = e / (D / 4), col = (e % (D / 4)) * 4, row = m & 15, w0 = m >> 4;
-        float mx = -INFINITY;
-        for (int k = 0; k < ng; k++) mx = fmaxf(mx, s.ml[w0 + k * wm][row].x);
+        float2 x[4];
+        float4 v[4];
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (k < ng) {
+                x[k] = s.ml[sx * 4 + w0 + k * wm][row];
+                v[k] = *reinterpret_cast<const float4*>(buf + ((w0 + k * wm) * 16 + row) * D + (((col >> 3) ^ (row & 7)) * 8 + (col & 7)));
+                mx = fmaxf(mx, x[k].x);
+            }
+        }
         const float off = mx == -INFINITY ? 0.f : mx;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-        for (int k = 0; k < ng; k++) {
-            const float2 x = s.ml[w0 + k * wm][row];
-            const float f = pf_ex2(x.x - off);
-            const float4 v = *reinterpret_cast<const float4*>(buf + ((w0 + k * wm) * 16 + row) * D + (((col >> 3) ^ (row & 7)) * 8 + (col & 7)));
-            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-            sum += x.y * f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (k < ng) {
+                const float f = pf_ex2(x[k].x - off);
+                acc.x += v[k].x * f; acc.y += v[k].y * f; acc.z += v[k].z * f; acc.w += v[k].w * f;
+                sum += x[k].y * f;
+            }
         }
-        *reinterpret_cast<float4*>(out + (long long)m * D + col) = acc;
+        *reinterpret_cast<float4*>(out + m * D + col) = acc;
         if (col == 0) ml[m] = make_float2(mx, sum);
     }
     __syncwarp();
-    if (lane == 0) pf_mbar_arrive(&s.join[1]);
+    if (lane == 0) pf_mbar_arrive(&s.njoin[sx]);
+    nn += 2;
     return true;
 }
 
@@ -415,14 +484,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < NST; i++) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 8); }
+        for (int i = 0; i < NST; i++) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 4); }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.qfull[i], 128);
             mbar_init(&s.sready[i], 1);
             mbar_init(&s.pready[i], 128);
             mbar_init(&s.odone[i], 1);
             mbar_init(&s.join[i], 8);
+            mbar_init(&s.njoin[i], 4);
+            mbar_init(&s.nturn[i], 4);
         }
+        for (int i = 0; i < kPfJobs; i++) { mbar_init(&s.jfull[i], 1); mbar_init(&s.jempty[i], 10); }
         mbar_fence_init();
         s.fail = 0;
     }
@@ -487,33 +559,24 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             }
             running += sum;
         }
-        __syncthreads();
-        const int i = tid - s.b0;      // (one chunk: the thread of a sequence still has its key count)
-        if (chunks == 1) {
-            if (i >= 0 && i < kPfWindow) s.keys[i] = keys;
-        } else if (tid < kPfWindow) {
-            s.keys[tid] = s.b0 + tid < a.seqs ? pf_own_keys(a, s.b0 + tid) : 0;
-        }
     }
     pf_fence_before();
     __syncthreads();
     pf_fence_after();
     const uint32_t tmem = s.tmem;
-    const int P = s.P;
-    PfIter it;
-    it.init(p, s);
     PfJob j;
     bool ok = true;
+    int nth = 0;
 
     if (warp >= 8) {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfOtherRegs));
       if (warp == 8) {
         // ---------------------------------------------------------------- copies
         int n = 0;                                   // copies issued so far: stage n % NST
-        while (ok && it.next(p, s, j)) {
-            const int keys = j.own ? it.keys : P;
-            const int* list = j.own ? a.table + (long long)j.b * a.max_pages : a.prefix_pages;
-            const int pages = (keys + 63) / 64, nu = j.u1 - j.u0;
+        while (pf_next(s, j, nth, ok)) {
+            const int* list = j.own() ? a.table + (long long)j.b * a.max_pages : a.prefix_pages;
+            const int pages = (j.keys + 63) / 64, nu = j.u1 - j.u0;
+            const bool pairs = j.pairs();
             // page numbers of 32 pages (16 units) at a time, the next 32 already on their way
             int at = j.u0 * 2;
             int ids = at + lane < pages ? list[at + lane] : 0, nxt = at + 32 + lane < pages ? list[at + 32 + lane] : 0;
@@ -521,7 +584,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             // copies in the tensor core's order: copy c of the job is K or V of some unit
             for (int c = 0; c < 2 * nu && ok; c++) {
                 int i, isv;
-                if (j.tiles == 2 || j.narrow) { i = c >> 1; isv = c & 1; }
+                if (pairs) { i = c >> 1; isv = c & 1; }
                 else if (c == 0) { i = 0; isv = 0; }
                 else if (c == 2 * nu - 1) { i = nu - 1; isv = 1; }
                 else if (c & 1) { i = (c + 1) >> 1; isv = 0; }
@@ -571,10 +634,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             constexpr uint32_t idescO = idesc0 | (1u << 16) | (((uint32_t)D >> 3) << 17);   // V: columns are the N side
             int base = 0;                    // copies of the jobs before this one
             uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
-            while (ok && it.next(p, s, j)) {
-                const int nu = j.u1 - j.u0, steps = nu * j.tiles;
-                if (j.narrow) { base += 2 * nu; continue; }
-                const bool pairs = j.tiles == 2;
+            while (pf_next(s, j, nth, ok)) {
+                const int nu = j.u1 - j.u0, steps = nu * j.tiles();
+                if (j.narrow()) { base += 2 * nu; continue; }
+                const bool pairs = j.tiles() == 2;
                 auto score = [&](int i) {    // S of stream i & 1 = Q K^T of step i
                     const int sx = i & 1, c = base + pf_stage_k(pairs ? i >> 1 : i, pairs), st = c % NST;
                     if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; return; }
@@ -615,6 +678,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             }
             if (!ok) s.fail = 1;
         }
+      } else if (warp == 10) {
+        // ---------------------------------------------------------------- jobs
+        PfIter it;
+        it.init(p, s, lane);
+        for (bool more = true; more && ok; nth++) {
+            more = it.next(p, s, j);
+            const int q = nth % kPfJobs;
+            if (nth >= kPfJobs && !pf_wait(&s.jempty[q], (uint32_t)((nth / kPfJobs - 1) & 1))) { ok = false; break; }
+            if (lane == 0) {
+                s.jobs[q] = j;
+                pf_mbar_arrive(&s.jfull[q]);
+            }
+            __syncwarp();
+        }
+        if (!ok) s.fail = 1;
       }
     } else {
         // ---------------------------------------------------------------- softmax
@@ -624,31 +702,34 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         const uint32_t tS = tmem + quarter + sx * 128, tO = tmem + quarter + 256;
         const float sl2 = a.scale * 1.4426950408889634f;
         int base = 0;
-        uint32_t ns = 0, no = 0, nj = 0;
-        while (ok && it.next(p, s, j)) {
-            const int nu = j.u1 - j.u0, steps = nu * j.tiles;
-            const int keys = j.own ? it.keys : P;
-            if (nj > 0 && !pf_wait(&s.join[1], (nj - 1) & 1)) { ok = false; break; }   // the last job's exchange has been read
-            if (j.narrow) {
-                ok = pf_narrow<T, D>(p, s, j, keys, smem, ring, base, nj);
-                nj++;
+        uint32_t ns = 0, no = 0, nj = 0, nn = 0;
+        uint32_t turn = 0;                                         // narrow jobs seen
+        while (pf_next(s, j, nth, ok)) {
+            const int nu = j.u1 - j.u0, tiles = j.tiles(), steps = nu * tiles, keys = j.keys;
+            const bool own = j.own();
+            // what the last jobs left in the streams' Q has been read (pf_narrow looks at its own)
+            if (nj > 0 && !pf_wait(&s.join[1], (nj - 1) & 1)) { ok = false; break; }
+            if (j.narrow()) {
+                if ((int)(turn & 1) == sx) ok = pf_narrow<T, D>(p, s, j, smem + sx * TB, ring, base, turn, nn);
+                turn++;
                 base += 2 * nu;
                 continue;
             }
+            if (nn > 0 && !pf_wait(&s.njoin[sx], (nn - 1) & 1)) { ok = false; break; }
             const int mine = (steps + 1 - sx) / 2;                 // steps of this stream
             if (mine == 0) { base += 2 * nu; continue; }           // (one unit of one tile: the other stream alone)
             // this thread's (row, query head) pair: lane `row` of the tile
-            const int tile0 = (j.grp * 2 + (j.tiles == 2 ? sx : 0)) * 128, m = tile0 + row;
-            const int pairsOf = (j.own ? a.T : a.seqs * a.T) * p.G;
+            const int tile0 = (j.grp * 2 + (tiles == 2 ? sx : 0)) * 128, m = tile0 + row;
+            const int pairsOf = (own ? a.T : a.seqs * a.T) * p.G;
             const bool live = m < pairsOf;
             int see = 0x7FFFFFFF;                                  // keys it sees (a lane without a pair: zeros, never written)
             const bool work = __any_sync(0xffffffffu, live);
             if (work) {
-                const int r = (j.own ? j.b * a.T : 0) + m / p.G;
+                const int r = (own ? j.b * a.T : 0) + m / p.G;
                 long long qat = -1;
                 if (live) {
                     qat = r * a.q_row + (j.h * p.G + m % p.G) * a.q_head;
-                    see = j.own ? min(keys, max(0, a.lens[r])) : P;
+                    see = own ? min(keys, max(0, a.lens[r])) : keys;
                 }
                 // the warp's 32 rows of Q, D / 8 lanes a row, into the operand's swizzled layout
                 constexpr int LPR = D / 8, RPI = 32 / LPR;
@@ -670,7 +751,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
 
             float ref = -INFINITY, l = 0.f;                        // reference of the exponents (log2 units), sum
             for (int i = 0; i < mine && ok; i++) {
-                const int unit = j.tiles == 2 ? i : 2 * i + sx, key0 = (j.u0 + unit) * kPfKeys;
+                const int unit = tiles == 2 ? i : 2 * i + sx, key0 = (j.u0 + unit) * kPfKeys;
                 if (!pf_wait(&s.sready[sx], ns & 1)) { ok = false; break; }
                 ns++;
                 pf_fence_after();
@@ -725,8 +806,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 }
                 // values behind the last key may be anything, and 0 * NaN is NaN: their rows of the stage become zeros
                 const int kv = keys - key0;
-                if (kv < kPfKeys && (j.tiles == 1 || sx == 0)) {
-                    const int c = base + pf_stage_v(unit, nu, j.tiles == 2), st = c % NST;
+                if (kv < kPfKeys && (tiles == 1 || sx == 0)) {
+                    const int c = base + pf_stage_v(unit, nu, tiles == 2), st = c % NST;
                     if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; break; }
                     uint8_t* v = ring + (size_t)st * TB;
                     for (int e = kv * 8 + row; e < kPfKeys * 8; e += 128)
@@ -743,11 +824,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             if (!pf_wait(&s.odone[sx], no & 1)) { ok = false; break; }
             no++;
             pf_fence_after();
-            const bool join = j.tiles == 1 && steps > 1;           // both streams hold a part of the same tile
-            const int srow = (j.tiles == 2 ? sx * 128 : 0) + row;
-            const long long at = (long long)j.slot * (j.own ? p.rowsO : p.rowsP) + srow;
-            float2* ml = (j.own ? p.mlO : p.mlP) + at;
-            float* o = (j.own ? p.oO : p.oP) + at * D;
+            const bool join = tiles == 1 && steps > 1;           // both streams hold a part of the same tile
+            const int srow = (tiles == 2 ? sx * 128 : 0) + row;
+            const long long at = (long long)j.slot * (own ? p.rowsO : p.rowsP) + srow;
+            float2* ml = (own ? p.mlO : p.mlP) + at;
+            float* o = (own ? p.oO : p.oP) + at * D;
             if (!join) {
                 if (live) *ml = make_float2(ref, l);
                 if (work) {
