@@ -247,6 +247,28 @@ __device__ __forceinline__ float pf_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two fp32 operations an instruction
+__device__ __forceinline__ uint64_t pf_two(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void pf_split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t pf_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pf_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pf_mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 template <typename T> __device__ __forceinline__ uint32_t pf_pack(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pf_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf2(lo, hi); }
 template <> __device__ __forceinline__ uint32_t pf_pack<__half>(float lo, float hi) {
@@ -270,6 +292,22 @@ __device__ __forceinline__ void pf_st32(uint32_t addr, const uint32_t* r) {
         "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::PF_I8(r, 0),
         PF_I8(r, 8), PF_I8(r, 16), PF_I8(r, 24), "r"(addr)
         : "memory");
+}
+__device__ __forceinline__ void pf_ld8(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : PF_R8(r, 0) : "r"(addr));
+}
+__device__ __forceinline__ void pf_st8(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::PF_I8(r, 0), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pf_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : PF_R8(r, 0), PF_R8(r, 8)
+                 : "r"(addr));
+}
+__device__ __forceinline__ void pf_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::PF_I8(r, 0),
+                 PF_I8(r, 8), "r"(addr)
+                 : "memory");
 }
 __device__ __forceinline__ void pf_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pf_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -756,21 +794,31 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 ns++;
                 pf_fence_after();
                 if (work) {
+                    // scores this row does not see: -infinity, put into tensor memory eight columns at a time (the last
+                    // units of a job only; the code of the common path stays small enough for the instruction caches)
+                    const int nv = see - key0;
+                    if (__any_sync(0xffffffffu, nv < kPfKeys)) {
+                        const int first = max(0, __reduce_min_sync(0xffffffffu, nv)) & ~7;
+#pragma unroll 1
+                        for (int c = first; c < kPfKeys; c += 8) {
+                            uint32_t x[8];
+                            pf_ld8(tS + c, x);
+                            pf_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 8; e++) x[e] = c + e < nv ? x[e] : 0xFF800000u;
+                            pf_st8(tS + c, x);
+                        }
+                        pf_wait_st();
+                    }
                     uint32_t r[128];
 #pragma unroll
                     for (int c = 0; c < 4; c++) pf_ld32(tS + c * 32, r + c * 32);
                     pf_wait_ld();
-                    float x[128];
+                    float mx[4];
 #pragma unroll
-                    for (int c = 0; c < 128; c++) x[c] = __uint_as_float(r[c]);
-                    const int nv = see - key0;
-                    if (__any_sync(0xffffffffu, nv < kPfKeys)) {
+                    for (int c = 0; c < 4; c++) mx[c] = __uint_as_float(r[c]);
 #pragma unroll
-                        for (int c = 0; c < 128; c++) x[c] = c < nv ? x[c] : -INFINITY;
-                    }
-                    float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                    for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+                    for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(r[c]));
                     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
                     // O and l keep their reference until a score exceeds it by 2^8: then both move to the new maximum
                     float f = 1.f;
@@ -780,26 +828,31 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                     }
                     if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
                         l *= f;
-#pragma unroll
-                        for (int c = 0; c < D / 32; c++) {
-                            uint32_t o[32];
-                            pf_ld32(tO + sx * 128 + c * 32, o);
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            pf_ld16(tO + sx * 128 + c, o);
                             pf_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            pf_st32(tO + sx * 128 + c * 32, o);
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            pf_st16(tO + sx * 128 + c, o);
                         }
                     }
-                    const float off = ref == -INFINITY ? 0.f : ref;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float off = ref == -INFINITY ? 0.f : -ref;
+                    const uint64_t scale2 = pf_two(sl2, sl2), off2 = pf_two(off, off);
+                    uint64_t sum2[2] = {0, 0};
 #pragma unroll
                     for (int c = 0; c < 128; c += 2) {
-                        const float e0 = pf_ex2(fmaf(x[c], sl2, -off)), e1 = pf_ex2(fmaf(x[c + 1], sl2, -off));
-                        sum[c & 2] += e0;
-                        sum[(c & 2) + 1] += e1;
+                        float e0, e1;
+                        pf_split(pf_fma2(pf_two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, off2), e0, e1);
+                        e0 = pf_ex2(e0);
+                        e1 = pf_ex2(e1);
+                        sum2[(c >> 1) & 1] = pf_add2(sum2[(c >> 1) & 1], pf_two(e0, e1));
                         r[c >> 1] = pf_pack<T>(e0, e1);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    float s0, s1;
+                    pf_split(pf_add2(sum2[0], sum2[1]), s0, s1);
+                    l += s0 + s1;
                     pf_st32(tS, r);
                     pf_st32(tS + 32, r + 32);
                     pf_wait_st();
@@ -832,7 +885,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             if (!join) {
                 if (live) *ml = make_float2(ref, l);
                 if (work) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
                         uint32_t r[32];
                         pf_ld32(tO + sx * 128 + c * 32, r);
@@ -855,7 +908,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 const float f0 = pf_ex2(x0.x - off), f1 = pf_ex2(x1.x - off);
                 if (live && sx == 0) *ml = make_float2(mx, x0.y * f0 + x1.y * f1);
                 if (work) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 64; c++) {
                         const int col = sx * (D / 2) + c * 32;
                         uint32_t u[32], v[32];
