@@ -1026,7 +1026,10 @@ template <typename T, int D> cudaError_t pf_launch(const PfParams& p, int sms, c
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PfCfg<D>::kSmem); });
     if (e != cudaSuccess) return e;
-    e = vk_launch(attend_prefix_kernel<T, D>, dim3((unsigned)sms), dim3(kPfThreads), PfCfg<D>::kSmem, stream, p);
+    // Pairs of neighbours on the line of work as clusters, so that both SMs of a TPC run the same form: a CTA of the wide form
+    // beside one of the narrow form ran its softmax 1.1 to 1.25 times as long and its steps 1.4 times (the two loops do not
+    // fit the instruction cache that the SMs share).
+    e = vk_launch_cluster(attend_prefix_kernel<T, D>, dim3((unsigned)sms), dim3(kPfThreads), 2, PfCfg<D>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
     return vk_launch(attend_prefix_merge_kernel<T, D>, dim3((unsigned)(p.a.seqs * p.a.T * p.a.Hq)), dim3(128), 0, stream, p);
 }
@@ -1053,7 +1056,7 @@ int prefix_args_ok(const vk_prefix_args* a) {
     return VK_OK;
 }
 
-// One CTA per SM (148, the target's count, where no device answers).
+// One CTA per SM (148, the target's count, where no device answers), an even number.
 int pf_ctas() {
     static std::atomic<int> sms{0};
     int n = sms.load(std::memory_order_acquire);
@@ -1063,6 +1066,7 @@ int pf_ctas() {
             cudaGetLastError();
             return 148;
         }
+        n = n < 2 ? 2 : n & ~1;
         sms.store(n, std::memory_order_release);
     }
     return n;
