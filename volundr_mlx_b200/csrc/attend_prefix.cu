@@ -61,7 +61,8 @@ struct PfParams {
     int narrowP, narrowO;      // the form of either part
     PfCost costP, costO;
     int rowsP, rowsO;          // rows of a slot (a slot holds one job's partial result of one CTA)
-    int *head, *cum;           // workspace: {total, CTAs, prefix length, end of the prefix jobs}; where a sequence's jobs begin
+    int longest;               // longest unit
+    int *head, *cum;           // workspace: {share, longer shares, prefix length}; where a sequence's jobs begin
     float2 *mlP, *mlO;         // running maximum (log2 units) and sum
     float *oP, *oO;            // unnormalised output
 };
@@ -75,12 +76,16 @@ struct PfJob {
     __device__ __forceinline__ bool pairs() const { return kind & 6; }     // order of the job's copies (below)
 };
 
-// CTA c's interval of the line: equal shares, the first total % n one longer
-__device__ __forceinline__ int pf_low(int c, int total, int n) { return c * (total / n) + min(c, total % n); }
-__device__ __forceinline__ int pf_cta_of(int x, int total, int n) {
-    const int q = total / n, r = total % n, edge = r * (q + 1);
-    return x < edge ? x / (q + 1) : r + (x - edge) / q;
-}
+// The line dealt to n CTAs: equal shares, the first `rem` one longer. No share is shorter than the longest unit (n is chosen
+// so), hence every CTA between those of a job's first and last unit has a unit of it.
+struct PfDeal {
+    int q, rem;
+    __device__ __forceinline__ int low(int c) const { return c * q + min(c, rem); }
+    __device__ __forceinline__ int cta_of(int x) const {
+        const int edge = rem * (q + 1);
+        return x < edge ? x / (q + 1) : rem + (x - edge) / q;
+    }
+};
 
 // Units of a job that begin (behind its fixed part) inside [lo, hi), both relative to the job's start
 __device__ __forceinline__ void pf_units(int fixed, int w, int nu, int lo, int hi, int& u0, int& u1) {
@@ -574,17 +579,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         int all = 0;
         for (int c = 0; c < chunks; c++) all += scan(c);
         const int base = PfHead(p.MT, pf_nu(s.P), p.costP).len * a.KVH, total = base + all;
-        // (no more CTAs than shares of one unit)
-        const int n = min((int)gridDim.x, total / min(p.costP.one, p.costO.one));
+        const int n = max(1, min((int)gridDim.x, total / p.longest));
+        const PfDeal deal = {total / n, total % n};
         const bool has = (int)blockIdx.x < n;
-        const int lo = has ? pf_low(blockIdx.x, total, n) : total, hi = has ? pf_low(blockIdx.x + 1, total, n) : total;
+        const int lo = has ? deal.low(blockIdx.x) : total, hi = has ? deal.low(blockIdx.x + 1) : total;
         const int start = max(lo, base);
         if (tid == 0) {
             s.lo = lo;
             s.hi = hi;
             s.b0 = a.seqs;
             s.cb0 = total;
-            if (blockIdx.x == 0) { p.head[0] = total; p.head[1] = n; p.head[2] = P; p.head[3] = base; }
+            if (blockIdx.x == 0) { p.head[0] = deal.q; p.head[1] = deal.rem; p.head[2] = P; }
         }
         __syncthreads();
         int running = base;
@@ -937,67 +942,110 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
     if (tid == 0 && s.fail) vk_set_status(VK_ST_MBAR_TIMEOUT);
 }
 
-// out = sum of the pieces of a (row, query head) pair, in the order of the line of work: one CTA per pair, four warps share
-// the pieces.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_prefix_merge_kernel(const __grid_constant__ PfParams p) {
+// The pieces of one pair's prefix or own part: those of CTAs c0 .. c1 of the line, in the slots' rows at + c * step
+struct PfPieces {
+    int c0, c1;
+    long long at;
+};
+__device__ __forceinline__ PfPieces pf_pieces(const PfParams& p, bool own, int b, int m, int h, const PfDeal& deal) {
+    const vk_prefix_args& a = p.a;
+    const int tiles = own ? p.ST : p.MT, grp = m / 256;
+    const PfCost& cost = own ? p.costO : p.costP;
+    const PfHead hd(tiles, pf_nu(own ? pf_own_keys(a, b) : p.head[2]), cost);
+    const int w = 2 * grp + 1 < tiles ? cost.two : cost.one, first = (own ? p.cum[b] : 0) + h * hd.len + grp * hd.len2 + cost.fixed;
+    PfPieces x = {0, -1, (long long)((b * a.KVH + h) * hd.groups + grp) * (own ? p.rowsO : p.rowsP) + m - grp * 256};
+    if (hd.nu > 0) {
+        x.c0 = deal.cta_of(first);
+        x.c1 = deal.cta_of(first + w * (hd.nu - 1));
+    }
+    return x;
+}
+
+// out = sum of the pieces of a (row, query head) pair, in the order of the line of work. SPLIT: the eight warps of a CTA share one
+// pair's pieces (few pairs: a prefix that all SMs worked on has up to 148 of them); else a warp takes a pair. Both
+// are bound by the round trip lengths -> pieces -> sums, four pieces in flight a warp.
+template <typename T, int D, bool SPLIT>
+__global__ void __launch_bounds__(256) attend_prefix_merge_kernel(const __grid_constant__ PfParams p) {
     constexpr int E = D / 32;
-    __shared__ float so[4][D];
-    __shared__ float2 sml[4];
+    struct Vec { float v[E]; };
+    __shared__ float so[SPLIT ? 8 : 1][D];
+    __shared__ float2 sml[8];
     pdl_wait();
     pdl_launch_dependents();
     const vk_prefix_args& a = p.a;
-    const int r = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq, h = hq / p.G, g = hq % p.G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int pair = SPLIT ? blockIdx.x : blockIdx.x * 8 + warp;
+    if (pair >= a.seqs * a.T * a.Hq) return;
+    const int r = pair / a.Hq, hq = pair % a.Hq, h = hq / p.G, g = hq % p.G, b = r / a.T;
     if (a.lens[r] < 0) return;
-    const int total = p.head[0], n = p.head[1], P = p.head[2];
+    const PfDeal deal = {p.head[0], p.head[1]};
     float m = -INFINITY, l = 0.f, o[E] = {};
+#pragma unroll 1
     for (int own = 0; own < 2; own++) {
-        const int b = own ? r / a.T : 0, mm = (own ? r - b * a.T : r) * p.G + g, grp = mm / 256;
-        const PfCost& cost = own ? p.costO : p.costP;
-        const int tiles = own ? p.ST : p.MT;
-        const PfHead hd(tiles, pf_nu(own ? pf_own_keys(a, b) : P), cost);
-        if (hd.nu == 0) continue;
-        const int w = 2 * grp + 1 < tiles ? cost.two : cost.one;
-        const int A = (own ? p.cum[b] : 0) + h * hd.len + grp * hd.len2, B = A + cost.fixed + w * hd.nu;
-        const int slot = (b * a.KVH + h) * hd.groups + grp, srow = mm - grp * 256;
-        const int c0 = pf_cta_of(A, total, n), c1 = pf_cta_of(B - 1, total, n);
+        const PfPieces x = own ? pf_pieces(p, true, b, (r - b * a.T) * p.G + g, h, deal) : pf_pieces(p, false, 0, r * p.G + g, h, deal);
         const long long step = own ? p.rowsO : p.rowsP;
-        const float2* mls = (own ? p.mlO : p.mlP) + slot * step + srow;
-        const float* os = (own ? p.oO : p.oP) + (slot * step + srow) * D + lane;
-        for (int c = c0 + warp; c <= c1; c += 4) {
-            int u0, u1;
-            pf_units(cost.fixed, w, hd.nu, max(pf_low(c, total, n), A) - A, min(pf_low(c + 1, total, n), B) - A, u0, u1);
-            if (u1 <= u0) continue;
-            const float2 x = mls[c * step];
-            float v[E];
+        const float2* mls = (own ? p.mlO : p.mlP) + x.at;
+        const float* os = (own ? p.oO : p.oP) + x.at * D + lane * E;
+        constexpr int STRIDE = SPLIT ? 8 : 1;
+        for (int c = x.c0 + (SPLIT ? warp : 0); c <= x.c1; c += 4 * STRIDE) {
+            float2 ml[4];
+            Vec v[4];
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] = os[c * step * D + e * 32];
-            const float mn = fmaxf(m, x.x), off = mn == -INFINITY ? 0.f : mn;
-            const float f0 = exp2f(m - off), f1 = exp2f(x.x - off);
-            l = l * f0 + x.y * f1;
+            for (int k = 0; k < 4; k++) {
+                const int cc = c + k * STRIDE;
+                ml[k] = make_float2(-INFINITY, 0.f);
+                if (cc <= x.c1) {
+                    ml[k] = mls[cc * step];
+                    if constexpr (E == 4) *reinterpret_cast<float4*>(&v[k]) = *reinterpret_cast<const float4*>(os + cc * step * D);
+                    else *reinterpret_cast<float2*>(&v[k]) = *reinterpret_cast<const float2*>(os + cc * step * D);
+                } else {
 #pragma unroll
-            for (int e = 0; e < E; e++) o[e] = o[e] * f0 + v[e] * f1;
+                    for (int e = 0; e < E; e++) v[k].v[e] = 0.f;
+                }
+            }
+            const float mn = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), off = mn == -INFINITY ? 0.f : mn;
+            const float f0 = exp2f(m - off);
+            l *= f0;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] *= f0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float f = exp2f(ml[k].x - off);
+                l += ml[k].y * f;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] += v[k].v[e] * f;
+            }
             m = mn;
         }
     }
-    if (lane == 0) sml[warp] = make_float2(m, l);
+    if constexpr (SPLIT) {
+        if (lane == 0) sml[warp] = make_float2(m, l);
 #pragma unroll
-    for (int e = 0; e < E; e++) so[warp][e * 32 + lane] = o[e];
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= D) return;
-    float mx = -INFINITY, sum = 0.f, v = 0.f;
-    for (int i = 0; i < 4; i++) mx = fmaxf(mx, sml[i].x);
-    const float off = mx == -INFINITY ? 0.f : mx;
-    for (int i = 0; i < 4; i++) {
-        const float f = exp2f(sml[i].x - off);
-        sum += sml[i].y * f;
-        v += so[i][d] * f;
+        for (int e = 0; e < E; e++) so[warp][lane * E + e] = o[e];
+        __syncthreads();
+        if (warp != 0) return;
+        float mx = -INFINITY;
+        for (int i = 0; i < 8; i++) mx = fmaxf(mx, sml[i].x);
+        const float off = mx == -INFINITY ? 0.f : mx;
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.f;
+        for (int i = 0; i < 8; i++) {
+            const float f = exp2f(sml[i].x - off);
+            l += sml[i].y * f;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] += so[i][lane * E + e] * f;
+        }
     }
-    v = sum == 0.f ? 0.f : v / sum;                                // (no visible key: zeros)
-    if (a.gate) v /= 1.f + expf(-to_f(((const T*)a.gate)[r * a.gate_row + hq * a.gate_head + d]));
-    ((T*)a.out)[r * a.out_row + hq * a.out_head + d] = from_f<T>(v);
+    struct alignas(E * 2) Out { T v[E]; } y, gt;
+    if (a.gate) gt = *reinterpret_cast<const Out*>((const T*)a.gate + r * a.gate_row + hq * a.gate_head + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        float v = l == 0.f ? 0.f : o[e] / l;                       // (no visible key: zeros)
+        if (a.gate) v /= 1.f + expf(-to_f(gt.v[e]));
+        y.v[e] = from_f<T>(v);
+    }
+    *reinterpret_cast<Out*>((T*)a.out + r * a.out_row + hq * a.out_head + lane * E) = y;
 }
 
 typedef CUresult (*PfEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -1031,7 +1079,10 @@ template <typename T, int D> cudaError_t pf_launch(const PfParams& p, int sms, c
     // fit the instruction cache that the SMs share).
     e = vk_launch_cluster(attend_prefix_kernel<T, D>, dim3((unsigned)sms), dim3(kPfThreads), 2, PfCfg<D>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
-    return vk_launch(attend_prefix_merge_kernel<T, D>, dim3((unsigned)(p.a.seqs * p.a.T * p.a.Hq)), dim3(128), 0, stream, p);
+    // (a warp a pair from about four warps an SM on: attend of 16 rows x 40 heads takes MERGE_A us, MERGE_B with split pieces)
+    const int pairs = p.a.seqs * p.a.T * p.a.Hq;
+    if (pairs <= 4 * sms) return vk_launch(attend_prefix_merge_kernel<T, D, true>, dim3((unsigned)pairs), dim3(256), 0, stream, p);
+    return vk_launch(attend_prefix_merge_kernel<T, D, false>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p);
 }
 
 int prefix_args_ok(const vk_prefix_args* a) {
@@ -1083,6 +1134,7 @@ size_t pf_layout(PfParams& p, const vk_prefix_args* a, uint8_t* ws, int ctas) {
     p.narrowP = mP <= kPfNarrow;
     p.narrowO = mO <= kPfNarrow;
     p.costP = p.costO = PfCost{4, 4, 8};
+    p.longest = max(p.MT > 1 ? p.costP.two : p.costP.one, p.ST > 1 ? p.costO.two : p.costO.one);
     p.rowsP = (int)(mP < 256 ? mP : 256);
     p.rowsO = (int)(mO < 256 ? mO : 256);
     const size_t slotsP = (size_t)a->KVH * ((p.MT + 1) / 2) + ctas, slotsO = (size_t)a->seqs * a->KVH * ((p.ST + 1) / 2) + ctas;
