@@ -44,6 +44,8 @@ constexpr int kPfTile = 128, kPfKeys = 128, kPfNarrow = 64;
 // 216 + 216 + 72 = 3 x 168
 constexpr int kPfThreads = 384;
 constexpr int kPfSoftmaxRegs = 216, kPfOtherRegs = 72;
+// Exponentials on the FMA pipe: of every kPfPolyOf pairs of scores the first kPfPoly
+constexpr int kPfPoly = 1, kPfPolyOf = 4;
 constexpr int kPfJobs = 4;               // jobs handed out ahead
 // Lengths on the line of work: a job's fixed part, a unit of one tile, of two tiles, of the narrow form
 struct PfCost { int fixed, one, two; };
@@ -119,11 +121,12 @@ __device__ __forceinline__ int pf_own_keys(const vk_prefix_args& a, int b) {
 __device__ __forceinline__ int pf_nu(int keys) { return (keys + kPfKeys - 1) / kPfKeys; }
 
 struct PfShared {
-    uint64_t full[10], empty[10], qfull[2], sready[2], pready[2], odone[2], join[2], njoin[2], nturn[2], jfull[kPfJobs], jempty[kPfJobs];
+    uint64_t full[10], empty[10], qfull[2], sready[2], pready[2], pready2[2], odone[2], join[2], njoin[2], nturn[2], jfull[kPfJobs], jempty[kPfJobs];
     PfJob jobs[kPfJobs];
     int lo, hi, cb0, b0, P, fail;
     uint32_t tmem;
     int red[kPfThreads / 32];
+    int keys[32];              // of the sequences from b0 on
     float2 ml[8][16];
 };
 
@@ -139,7 +142,8 @@ struct PfIter {
         prefixEnd = PfHead(p.MT, pf_nu(s.P), p.costP).len * p.a.KVH;
         cur = s.lo; hi = s.hi;
         b = s.b0; cb = s.cb0;
-        look(p, b);
+        window = b;
+        mine = s.keys[lane];
     }
     __device__ __forceinline__ bool next(const PfParams& p, const PfShared& s, PfJob& j) {
         while (cur < hi) {
@@ -274,6 +278,28 @@ __device__ __forceinline__ uint64_t pf_mul2(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+__device__ __forceinline__ float pf_max_nan(float a, float b) {   // NaN if either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x of two numbers on the FMA pipe, for a part of the exponentials (the special function unit does one warp's worth in
+// eight cycles): x = n + f by rounding, 2^f on [-1/2, 1/2] as the degree-4 polynomial of least relative error (2.7e-6 in fp32,
+// found by exchange iteration), n added to the exponent; zero below 2^-126.
+__device__ __forceinline__ void pf_ex2_poly(uint64_t x, float& e0, float& e1) {
+    const uint64_t r = pf_add2(x, pf_two(12582912.f, 12582912.f));        // 1.5 * 2^23: the integer in the low bits
+    const uint64_t f = pf_fma2(pf_add2(r, pf_two(-12582912.f, -12582912.f)), pf_two(-1.f, -1.f), x);
+    uint64_t q = pf_fma2(pf_two(0.009570102f, 0.009570102f), f, pf_two(0.05591786f, 0.05591786f));
+    q = pf_fma2(q, f, pf_two(0.24024745f, 0.24024745f));
+    q = pf_fma2(q, f, pf_two(0.6931218f, 0.6931218f));
+    q = pf_fma2(q, f, pf_two(0.99999926f, 0.99999926f));
+    float x0, x1, r0, r1, q0, q1;
+    pf_split(x, x0, x1);
+    pf_split(r, r0, r1);
+    pf_split(q, q0, q1);
+    e0 = x0 < -126.f ? 0.f : __uint_as_float(__float_as_uint(q0) + (__float_as_uint(r0) << 23));
+    e1 = x1 < -126.f ? 0.f : __uint_as_float(__float_as_uint(q1) + (__float_as_uint(r1) << 23));
+}
 template <typename T> __device__ __forceinline__ uint32_t pf_pack(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pf_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf2(lo, hi); }
 template <> __device__ __forceinline__ uint32_t pf_pack<__half>(float lo, float hi) {
@@ -313,6 +339,9 @@ __device__ __forceinline__ void pf_st16(uint32_t addr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::PF_I8(r, 0),
                  PF_I8(r, 8), "r"(addr)
                  : "memory");
+}
+__device__ __forceinline__ void pf_store8(float* p, const uint32_t* r) {   // 32 bytes: a whole sector per lane
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), PF_I8(r, 0) : "memory");
 }
 __device__ __forceinline__ void pf_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pf_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -532,6 +561,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             mbar_init(&s.qfull[i], 128);
             mbar_init(&s.sready[i], 1);
             mbar_init(&s.pready[i], 128);
+            mbar_init(&s.pready2[i], 128);
             mbar_init(&s.odone[i], 1);
             mbar_init(&s.join[i], 8);
             mbar_init(&s.njoin[i], 4);
@@ -602,6 +632,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             }
             running += sum;
         }
+        __syncthreads();
+        const int i = tid - s.b0;      // (one chunk: the thread of a sequence still has its key count)
+        if (chunks == 1) {
+            if (i >= 0 && i < 32) s.keys[i] = keys;
+        } else if (tid < 32) {
+            s.keys[tid] = s.b0 + tid < a.seqs ? pf_own_keys(a, s.b0 + tid) : 0;
+        }
     }
     pf_fence_before();
     __syncthreads();
@@ -633,6 +670,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 else if (c & 1) { i = (c + 1) >> 1; isv = 0; }
                 else { i = (c - 2) >> 1; isv = 1; }
                 const int st = n % NST;
+                // (the first job's Q is read before the ring's first load fills the memory system: behind it, it took up to 7 us)
+                if (n == 2 && nth == 1 && !j.narrow() && !pf_wait(&s.qfull[0], 0)) { ok = false; break; }
                 if (n >= NST && !pf_wait(&s.empty[st], (uint32_t)((n / NST - 1) & 1))) { ok = false; break; }
                 const int pg = (j.u0 + i) * 2, cnt = min(2, pages - pg);
                 // (V trails K by one unit: the window moves on only when V's pages are behind it, so look both up here)
@@ -705,14 +744,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                     const int sx = i & 1, unit = pairs ? i >> 1 : i;
                     const int c = base + pf_stage_v(unit, nu, pairs), st = c % NST;
                     if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1)) || !pf_wait(&s.pready[sx], np[sx] & 1)) { ok = false; break; }
-                    np[sx]++;
                     pf_fence_after();
                     const uint32_t v0 = smem_u32(ring + (size_t)st * TB);
 #pragma unroll
                     for (int kk = 0; kk < kPfKeys / 16; kk++) {
+                        if (kk == kPfKeys / 32) {                     // the second half of P
+                            if (!pf_wait(&s.pready2[sx], np[sx] & 1)) { ok = false; break; }
+                            pf_fence_after();
+                        }
                         const uint64_t db = pf_desc(v0 + kk * 2048, 16384);
                         pf_mma_ts(tmem + 256 + sx * 128, tmem + sx * 128 + kk * 8, db, idescO, i >= 2 || kk > 0 ? 1u : 0u);
                     }
+                    np[sx]++;
                     if (!pairs || sx == 1) pf_commit_stage(&s.empty[st]);
                     if (i + 2 >= steps) pf_commit(&s.odone[sx]);
                     else score(i + 2);
@@ -793,6 +836,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             pf_mbar_arrive(&s.qfull[sx]);
 
             float ref = -INFINITY, l = 0.f;                        // reference of the exponents (log2 units), sum
+            // values behind the last key may be anything, and 0 * NaN is NaN: their rows of the stage become zeros
+            auto clear_values = [&](int key0, int unit) {
+                const int kv = keys - key0;
+                if (kv < kPfKeys && (tiles == 1 || sx == 0)) {
+                    const int c = base + pf_stage_v(unit, nu, tiles == 2), st = c % NST;
+                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) return false;
+                    uint8_t* v = ring + (size_t)st * TB;
+                    for (int e = kv * 8 + row; e < kPfKeys * 8; e += 128)
+#pragma unroll
+                        for (int x = 0; x < D / 64; x++) *reinterpret_cast<uint4*>(v + x * 16384 + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async_smem();
+                }
+                return true;
+            };
             for (int i = 0; i < mine && ok; i++) {
                 const int unit = tiles == 2 ? i : 2 * i + sx, key0 = (j.u0 + unit) * kPfKeys;
                 if (!pf_wait(&s.sready[sx], ns & 1)) { ok = false; break; }
@@ -816,18 +873,19 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                         pf_wait_st();
                     }
                     uint32_t r[128];
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    pf_ld32(tS, r);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) pf_ld32(tS + c * 32, r + c * 32);
-                    pf_wait_ld();
-                    float mx[4];
+                    for (int c = 1; c <= 4; c++) {
+                        pf_wait_ld();
+                        if (c < 4) pf_ld32(tS + c * 32, r + c * 32);
 #pragma unroll
-                    for (int c = 0; c < 4; c++) mx[c] = __uint_as_float(r[c]);
-#pragma unroll
-                    for (int c = 4; c < 128; c++) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(r[c]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                        for (int e = 0; e < 32; e++) mx[e & 3] = pf_max_nan(mx[e & 3], __uint_as_float(r[(c - 1) * 32 + e]));
+                    }
+                    const float top = pf_max_nan(pf_max_nan(mx[0], mx[1]), pf_max_nan(mx[2], mx[3])) * sl2;
                     // O and l keep their reference until a score exceeds it by 2^8: then both move to the new maximum
                     float f = 1.f;
-                    if (top > ref + 8.f || ref == -INFINITY) {
+                    if (!(top <= ref + 8.f) || ref == -INFINITY) {        // (a NaN score makes the whole row NaN)
                         if (ref != -INFINITY) f = pf_ex2(ref - top);
                         ref = top;
                     }
@@ -846,35 +904,40 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                     const float off = ref == -INFINITY ? 0.f : -ref;
                     const uint64_t scale2 = pf_two(sl2, sl2), off2 = pf_two(off, off);
                     uint64_t sum2[2] = {0, 0};
+                    // P in two halves, so that the tensor core begins with the first while the second is made
 #pragma unroll
-                    for (int c = 0; c < 128; c += 2) {
-                        float e0, e1;
-                        pf_split(pf_fma2(pf_two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, off2), e0, e1);
-                        e0 = pf_ex2(e0);
-                        e1 = pf_ex2(e1);
-                        sum2[(c >> 1) & 1] = pf_add2(sum2[(c >> 1) & 1], pf_two(e0, e1));
-                        r[c >> 1] = pf_pack<T>(e0, e1);
+                    for (int half = 0; half < 2; half++) {
+#pragma unroll
+                        for (int c = half * 64; c < half * 64 + 64; c += 2) {
+                            float e0, e1;
+                            const uint64_t x = pf_fma2(pf_two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, off2);
+                            if ((c >> 1) % kPfPolyOf < kPfPoly) {
+                                pf_ex2_poly(x, e0, e1);
+                            } else {
+                                pf_split(x, e0, e1);
+                                e0 = pf_ex2(e0);
+                                e1 = pf_ex2(e1);
+                            }
+                            sum2[(c >> 1) & 1] = pf_add2(sum2[(c >> 1) & 1], pf_two(e0, e1));
+                            r[c >> 1] = pf_pack<T>(e0, e1);
+                        }
+                        pf_st32(tS + half * 32, r + half * 32);
+                        pf_wait_st();
+                        if (half == 0) {
+                            if (!clear_values(key0, unit)) { ok = false; break; }
+                            pf_fence_before();
+                            pf_mbar_arrive(&s.pready[sx]);
+                        }
                     }
                     float s0, s1;
                     pf_split(pf_add2(sum2[0], sum2[1]), s0, s1);
                     l += s0 + s1;
-                    pf_st32(tS, r);
-                    pf_st32(tS + 32, r + 32);
-                    pf_wait_st();
-                }
-                // values behind the last key may be anything, and 0 * NaN is NaN: their rows of the stage become zeros
-                const int kv = keys - key0;
-                if (kv < kPfKeys && (tiles == 1 || sx == 0)) {
-                    const int c = base + pf_stage_v(unit, nu, tiles == 2), st = c % NST;
-                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; break; }
-                    uint8_t* v = ring + (size_t)st * TB;
-                    for (int e = kv * 8 + row; e < kPfKeys * 8; e += 128)
-#pragma unroll
-                        for (int x = 0; x < D / 64; x++) *reinterpret_cast<uint4*>(v + x * 16384 + e * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    fence_proxy_async_smem();
+                } else {
+                    if (!clear_values(key0, unit)) { ok = false; break; }
+                    pf_mbar_arrive(&s.pready[sx]);
                 }
                 pf_fence_before();
-                pf_mbar_arrive(&s.pready[sx]);
+                pf_mbar_arrive(&s.pready2[sx]);
             }
             base += 2 * nu;
             if (!ok) break;
@@ -897,7 +960,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                         pf_wait_ld();
                         if (live) {
 #pragma unroll
-                            for (int e = 0; e < 8; e++) reinterpret_cast<uint4*>(o)[c * 8 + e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                            for (int e = 0; e < 32; e += 8) pf_store8(o + c * 32 + e, r + e);
                         }
                     }
                 }
@@ -924,7 +987,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
 #pragma unroll
                             for (int e = 0; e < 32; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * f0 + __uint_as_float(v[e]) * f1);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) reinterpret_cast<uint4*>(o + col)[e] = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
+                            for (int e = 0; e < 32; e += 8) pf_store8(o + col + e, u + e);
                         }
                     }
                 }
@@ -1081,7 +1144,7 @@ template <typename T, int D> cudaError_t pf_launch(const PfParams& p, int sms, c
     if (e != cudaSuccess) return e;
     // (a warp a pair from about four warps an SM on: attend of 16 rows x 40 heads takes MERGE_A us, MERGE_B with split pieces)
     const int pairs = p.a.seqs * p.a.T * p.a.Hq;
-    if (pairs <= 4 * sms) return vk_launch(attend_prefix_merge_kernel<T, D, true>, dim3((unsigned)pairs), dim3(256), 0, stream, p);
+    if (pairs <= 8 * sms) return vk_launch(attend_prefix_merge_kernel<T, D, true>, dim3((unsigned)pairs), dim3(256), 0, stream, p);
     return vk_launch(attend_prefix_merge_kernel<T, D, false>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p);
 }
 
