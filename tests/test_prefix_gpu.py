@@ -144,6 +144,17 @@ def test_many_rows(cuda):
     Case(40, 8, 128, 1500, [(13 * i) % 97 for i in range(128)], seed=13).check()
 
 
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 1), (64, 5)])
+def test_many_jobs_a_processor(cuda, D, T):
+    """Jobs of two tiles, of one tile and of few rows follow one another on every processor, many times over."""
+    S = 300 // T
+    lens = []
+    for i in range(S):
+        lens += [max(0, (29 * i) % 300 - T + 1 + t) for t in range(T)]
+    Case(200, 200, D, 300, lens, T=T, seed=19).check()
+    Case(390, 3, D, 130, lens[: 20 * T], T=T, seed=20).check()
+
+
 def test_same_bits_every_time(cuda):
     c = Case(40, 8, 128, 3000, [5, 900, 64, 65, 1, 0, 2000], seed=14)
     a = c.run().clone()

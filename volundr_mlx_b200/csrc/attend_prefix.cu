@@ -31,7 +31,8 @@ namespace {
 // A unit of work is 128 keys of one kv head against a tile of (row, query head) pairs. Two forms:
 //   wide   up to 128 pairs, one tensor-memory lane each: S[128 x 128] = Q K^T (tcgen05.mma, Q and K in shared memory),
 //          P = exp2(S - m) in registers, O[128 x D] += P V with P in tensor memory (over S) and V in shared memory. Two
-//          streams (softmax warpgroups) take turns on the tensor core: two tiles on the same keys, or one tile's even and odd units;
+//          streams (a softmax warpgroup and a warp that issues its MMAs each) share the tensor core: two tiles on the same keys,
+//          or one tile on the two 64-key halves of every unit;
 //   narrow up to 64 pairs (a sequence's own keys, a small batch): mma.sync m16n8k16 by one warpgroup, the unit's keys dealt to
 //          its warps in chunks of 32, each warp with its own running maximum, sum and output, joined when the job ends.
 //          The two warpgroups take jobs in turn, so that one's start and end lie under the other's units. No round trips
@@ -39,9 +40,9 @@ namespace {
 // A job is a run of units: a tile, or two tiles that share the keys, against the prefix or against one sequence's own keys.
 // All jobs lie on one line, each as long as it is expected to take, and every CTA takes an equal interval of it.
 constexpr int kPfTile = 128, kPfKeys = 128, kPfNarrow = 64;
-// warps 0-3 and 4-7: softmax of two streams; 8: copies; 9: tensor core; 10: walks the line of work and hands out the jobs; 11
-// fills the third warpgroup, whose registers go to the softmax (a row of S is 128 registers): 168 a thread at launch, then
-// 216 + 216 + 72 = 3 x 168
+// warps 0-3 and 4-7: softmax of two streams; 8: copies; 9, 11: MMAs of the streams (one warp for both took 4400 cycles for what the
+// tensor core does in 2050: its own instructions were the limit); 10: walks the line of work and hands out the jobs. The
+// third warpgroup's registers go to the softmax (a row of S is 128 registers): 168 a thread at launch, then 216 + 216 + 72
 constexpr int kPfThreads = 384;
 constexpr int kPfSoftmaxRegs = 216, kPfOtherRegs = 72;
 // Exponentials on the FMA pipe: of every kPfPolyOf pairs of scores the first kPfPoly
@@ -75,7 +76,6 @@ struct PfJob {
     __device__ __forceinline__ bool own() const { return kind & 1; }
     __device__ __forceinline__ int tiles() const { return kind & 2 ? 2 : 1; }
     __device__ __forceinline__ bool narrow() const { return kind & 4; }
-    __device__ __forceinline__ bool pairs() const { return kind & 6; }     // order of the job's copies (below)
 };
 
 // The line dealt to n CTAs: equal shares, the first `rem` one longer. No share is shorter than the longest unit (n is chosen
@@ -121,7 +121,7 @@ __device__ __forceinline__ int pf_own_keys(const vk_prefix_args& a, int b) {
 __device__ __forceinline__ int pf_nu(int keys) { return (keys + kPfKeys - 1) / kPfKeys; }
 
 struct PfShared {
-    uint64_t full[10], empty[10], qfull[2], sready[2], pready[2], pready2[2], odone[2], join[2], njoin[2], nturn[2], jfull[kPfJobs], jempty[kPfJobs];
+    uint64_t full[10], empty[10], qfull[2], sready[2][2], pready[2][2], pvdone[2], join[2], njoin[2], nturn[2], jfull[kPfJobs], jempty[kPfJobs];
     PfJob jobs[kPfJobs];
     int lo, hi, cb0, b0, P, fail;
     uint32_t tmem;
@@ -183,11 +183,6 @@ struct PfIter {
     }
 };
 
-// Order of a job's copies in the stage ring. pairs: K and V of one unit after another (two tiles; narrow jobs); else the tensor
-// core runs two score products ahead of the values.
-__device__ __forceinline__ int pf_stage_k(int i, bool pairs) { return pairs ? 2 * i : (i == 0 ? 0 : 2 * i - 1); }
-__device__ __forceinline__ int pf_stage_v(int i, int n, bool pairs) { return pairs ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2); }
-
 __device__ __forceinline__ void pf_mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -203,34 +198,42 @@ __device__ __forceinline__ bool pf_next(PfShared& s, PfJob& j, int& nth, bool& o
     nth++;
     return j.kind >= 0;
 }
-// (whole-warp calls, one elected lane acts: the operands stay warp-uniform)
+// The calls from here to pf_mma_pv are a whole warp's and one elected lane acts: with warp-uniform operands eight MMAs take 520
+// cycles to issue, and 560 to 600 beside the softmax warps of the same scheduler; from inside a branch on the lane,
+// 560, and 780 to 950.
+#define PF_ELECT ".reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
 __device__ __forceinline__ void pf_commit(uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
-        : "memory");
+    asm volatile("{\n\t" PF_ELECT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)) : "memory");
 }
-// A stage's "empty" barrier counts the four warps of the narrow form: three arrivals now, the fourth when the MMAs are done
+// A stage's "empty" barrier counts the four warps of the narrow form; of the wide form's two streams each arrives once now and
+// once when its MMAs are done
 __device__ __forceinline__ void pf_commit_stage(uint64_t* bar) {
     asm volatile(
-        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e mbarrier.arrive.shared::cta.b64 _, [%0], 3;\n\t"
+        "{\n\t" PF_ELECT "@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t"
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
         : "memory");
 }
-__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+// S = Q K^T: descriptors step 32 bytes (16 elements) inside a block of 64 columns, 16 KB to the next
+#define PF_QK(off) "add.u64 a, %1, " #off ";\n\tadd.u64 b, %2, " #off ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, t;\n\t"
+template <int D> __device__ __forceinline__ void pf_mma_qk(uint32_t d, uint64_t q, uint64_t k, uint32_t idesc) {
+    if constexpr (D == 128)
+        asm volatile("{\n\t.reg .pred f, t;\n\t.reg .b64 a, b;\n\tsetp.eq.b32 f, %3, 0;\n\tsetp.ne.b32 t, %3, 0;\n\t" PF_ELECT
+                     "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, f;\n\t" PF_QK(2) PF_QK(4) PF_QK(6) PF_QK(1024) PF_QK(1026)
+                         PF_QK(1028) PF_QK(1030) "}" ::"r"(d), "l"(q), "l"(k), "r"(idesc)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred f, t;\n\t.reg .b64 a, b;\n\tsetp.eq.b32 f, %3, 0;\n\tsetp.ne.b32 t, %3, 0;\n\t" PF_ELECT
+                     "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, f;\n\t" PF_QK(2) PF_QK(4) PF_QK(6) "}" ::"r"(d), "l"(q),
+                     "l"(k), "r"(idesc)
+                     : "memory");
 }
-__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(ta), "l"(db), "r"(idesc), "r"(accumulate)
-        : "memory");
+// O (+)= P V over 64 keys: P advances 8 columns of tensor memory, V 16 rows (2 KB) a step
+#define PF_PV(pa, vb) "add.u32 a, %1, " #pa ";\n\tadd.u64 b, %2, " #vb ";\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+__device__ __forceinline__ void pf_mma_pv(uint32_t d, uint32_t pm, uint64_t v, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred f, t;\n\t.reg .b64 b;\n\t.reg .b32 a;\n\tsetp.ne.b32 f, %4, 0;\n\tsetp.ne.b32 t, %3, 0;\n\t" PF_ELECT
+                 "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, f;\n\t" PF_PV(8, 128) PF_PV(16, 256) PF_PV(24, 384) "}" ::"r"(d),
+                 "r"(pm), "l"(v), "r"(idesc), "r"(accumulate)
+                 : "memory");
 }
 __device__ __forceinline__ void pf_ldm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -352,6 +355,86 @@ __device__ __forceinline__ void pf_fence_after() { asm volatile("tcgen05.fence::
 // bytes between blocks of 64 columns (used where the columns are the operand's M or N side)
 __device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// One step of a stream's softmax (a warp, its lanes' rows of S in tensor memory at tS): 64 scores a row become probabilities,
+// in place. nv: scores of the step that the row sees; settled(): waits until the product before has been added to O.
+template <typename T, int D, typename Settled>
+__device__ __forceinline__ bool pf_softmax(uint32_t tS, uint32_t tO, int nv, bool first, float sl2, float& ref, float& l, Settled settled) {
+    constexpr int N = 64;
+    // scores the row does not see: -infinity, put into tensor memory eight columns at a time (the last units of a job
+    // only; the code of the common path stays small enough for the instruction caches)
+    if (__any_sync(0xffffffffu, nv < N)) {
+#pragma unroll 1
+        for (int c = max(0, __reduce_min_sync(0xffffffffu, nv)) & ~7; c < N; c += 8) {
+            uint32_t x[8];
+            pf_ld8(tS + c, x);
+            pf_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = c + e < nv ? x[e] : 0xFF800000u;
+            pf_st8(tS + c, x);
+        }
+        pf_wait_st();
+    }
+    uint32_t r[N];
+    float mx[8];
+    pf_ld32(tS, r);
+    pf_wait_ld();
+    pf_ld32(tS + 32, r + 32);
+#pragma unroll
+    for (int e = 0; e < 8; e++) mx[e] = __uint_as_float(r[e]);
+#pragma unroll
+    for (int e = 8; e < 32; e++) mx[e & 7] = pf_max_nan(mx[e & 7], __uint_as_float(r[e]));
+    pf_wait_ld();
+#pragma unroll
+    for (int e = 32; e < 64; e++) mx[e & 7] = pf_max_nan(mx[e & 7], __uint_as_float(r[e]));
+#pragma unroll
+    for (int e = 4; e > 0; e >>= 1)
+#pragma unroll
+        for (int k = 0; k < e; k++) mx[k] = pf_max_nan(mx[k], mx[k + e]);
+    const float top = mx[0] * sl2;
+    // O and l keep their reference until a score exceeds it by 2^8: then both move to the new maximum
+    float f = 1.f;
+    if (!(top <= ref + 8.f) || ref == -INFINITY) {        // (a NaN score makes the whole row NaN)
+        if (ref != -INFINITY) f = pf_ex2(ref - top);
+        ref = top;
+    }
+    if (!first && __any_sync(0xffffffffu, f != 1.f)) {
+        if (!settled()) return false;
+        l *= f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            pf_ld16(tO + c, o);
+            pf_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            pf_st16(tO + c, o);
+        }
+    }
+    const float off = ref == -INFINITY ? 0.f : -ref;
+    const uint64_t scale2 = pf_two(sl2, sl2), off2 = pf_two(off, off);
+    uint64_t sum2[2] = {0, 0};
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+        float e0, e1;
+        const uint64_t x = pf_fma2(pf_two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, off2);
+        if ((c >> 1) % kPfPolyOf < kPfPoly) {
+            pf_ex2_poly(x, e0, e1);
+        } else {
+            pf_split(x, e0, e1);
+            e0 = pf_ex2(e0);
+            e1 = pf_ex2(e1);
+        }
+        sum2[(c >> 1) & 1] = pf_add2(sum2[(c >> 1) & 1], pf_two(e0, e1));
+        r[c >> 1] = pf_pack<T>(e0, e1);
+    }
+    pf_st32(tS, r);
+    float s0, s1;
+    pf_split(pf_add2(sum2[0], sum2[1]), s0, s1);
+    l += s0 + s1;
+    pf_wait_st();
+    return true;
 }
 
 // A narrow job, by one warpgroup: 16-row tile warp % wm of the pairs, keys of chunks warp / wm, + 4 / wm, ... of every unit.
@@ -559,15 +642,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         for (int i = 0; i < NST; i++) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 4); }
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.qfull[i], 128);
-            mbar_init(&s.sready[i], 1);
-            mbar_init(&s.pready[i], 128);
-            mbar_init(&s.pready2[i], 128);
-            mbar_init(&s.odone[i], 1);
+            for (int b = 0; b < 2; b++) {
+                mbar_init(&s.sready[i][b], 1);
+                mbar_init(&s.pready[i][b], 128);
+            }
+            mbar_init(&s.pvdone[i], 1);
             mbar_init(&s.join[i], 8);
             mbar_init(&s.njoin[i], 4);
             mbar_init(&s.nturn[i], 4);
         }
-        for (int i = 0; i < kPfJobs; i++) { mbar_init(&s.jfull[i], 1); mbar_init(&s.jempty[i], 10); }
+        for (int i = 0; i < kPfJobs; i++) { mbar_init(&s.jfull[i], 1); mbar_init(&s.jempty[i], 11); }
         mbar_fence_init();
         s.fail = 0;
     }
@@ -656,37 +740,24 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         while (pf_next(s, j, nth, ok)) {
             const int* list = j.own() ? a.table + (long long)j.b * a.max_pages : a.prefix_pages;
             const int pages = (j.keys + 63) / 64, nu = j.u1 - j.u0;
-            const bool pairs = j.pairs();
             // page numbers of 32 pages (16 units) at a time, the next 32 already on their way
             int at = j.u0 * 2;
             int ids = at + lane < pages ? list[at + lane] : 0, nxt = at + 32 + lane < pages ? list[at + 32 + lane] : 0;
             int ids0 = at;
-            // copies in the tensor core's order: copy c of the job is K or V of some unit
             for (int c = 0; c < 2 * nu && ok; c++) {
-                int i, isv;
-                if (pairs) { i = c >> 1; isv = c & 1; }
-                else if (c == 0) { i = 0; isv = 0; }
-                else if (c == 2 * nu - 1) { i = nu - 1; isv = 1; }
-                else if (c & 1) { i = (c + 1) >> 1; isv = 0; }
-                else { i = (c - 2) >> 1; isv = 1; }
+                const int i = c >> 1, isv = c & 1;
                 const int st = n % NST;
                 // (the first job's Q is read before the ring's first load fills the memory system: behind it, it took up to 7 us)
                 if (n == 2 && nth == 1 && !j.narrow() && !pf_wait(&s.qfull[0], 0)) { ok = false; break; }
                 if (n >= NST && !pf_wait(&s.empty[st], (uint32_t)((n / NST - 1) & 1))) { ok = false; break; }
                 const int pg = (j.u0 + i) * 2, cnt = min(2, pages - pg);
-                // (V trails K by one unit: the window moves on only when V's pages are behind it, so look both up here)
-                if (pg - ids0 >= 34) {
+                if (pg - ids0 >= 32) {
                     ids0 += 32;
                     ids = nxt;
                     nxt = ids0 + 32 + lane < pages ? list[ids0 + 32 + lane] : 0;
                 }
                 const int rel = pg - ids0;
-                int pid[2];
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int x = __shfl_sync(0xffffffffu, ids, (rel + k) & 31), y = __shfl_sync(0xffffffffu, nxt, (rel + k) & 31);
-                    pid[k] = rel + k < 32 ? x : y;
-                }
+                const int pid[2] = {__shfl_sync(0xffffffffu, ids, rel), __shfl_sync(0xffffffffu, ids, rel + 1)};
                 if (lane == 0) {
                     fence_proxy_async_smem();   // (rows behind the last key are zeroed in the generic proxy)
                     mbar_expect_tx(&s.full[st], (uint32_t)(cnt * 64 * D * 2));
@@ -707,60 +778,70 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             s.fail = 1;
             for (int k = n > NST ? n - NST : 0; k < n; k++) mbar_wait(&s.full[k % NST], (uint32_t)((k / NST) & 1));
         }
-      } else if (warp == 9) {
-        // ---------------------------------------------------------------- tensor core (the wide form)
+      } else if (warp != 10) {
+        // ---------------------------------------------------------------- tensor core (the wide form): a warp a stream
         {
             constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
             constexpr uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
-            constexpr uint32_t idescS = idesc0 | ((128u >> 3) << 17);
             constexpr uint32_t idescO = idesc0 | (1u << 16) | (((uint32_t)D >> 3) << 17);   // V: columns are the N side
-            int base = 0;                    // copies of the jobs before this one
-            uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+            const int sx = warp == 9 ? 0 : 1;
+            const uint32_t tS = tmem + sx * 128, tO = tmem + 256 + sx * 128;
+            const uint64_t q = pf_desc(smem_u32(smem + sx * TB), 16);
+            const uint64_t ring0 = pf_desc(smem_u32(ring), 16);
+            constexpr uint64_t kLead = (uint64_t)((16384 - 16) >> 4) << 16;                 // (V: blocks of 64 columns 16 KB apart)
+            constexpr uint32_t idescS = idesc0 | ((64u >> 3) << 17);
+            int st = 0;                      // the job's first copy: its stage and phase
+            uint32_t ph = 0, nq = 0, np[2] = {0, 0};
+            auto ahead = [](int& stage, uint32_t& phase, int n) {
+                stage += n;
+                phase ^= (uint32_t)((stage / NST) & 1);
+                stage %= NST;
+            };
             while (pf_next(s, j, nth, ok)) {
-                const int nu = j.u1 - j.u0, steps = nu * j.tiles();
-                if (j.narrow()) { base += 2 * nu; continue; }
-                const bool pairs = j.tiles() == 2;
-                auto score = [&](int i) {    // S of stream i & 1 = Q K^T of step i
-                    const int sx = i & 1, c = base + pf_stage_k(pairs ? i >> 1 : i, pairs), st = c % NST;
-                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; return; }
-                    pf_fence_after();
-                    const uint32_t q0 = smem_u32(smem + sx * TB), k0 = smem_u32(ring + (size_t)st * TB);
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; kk++) {
-                        const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                        const uint64_t da = pf_desc(q0 + off, 16), db = pf_desc(k0 + off, 16);
-                        pf_mma_ss(tmem + sx * 128, da, db, idescS, kk > 0 ? 1u : 0u);
-                    }
-                    if (!pairs || sx == 1) pf_commit_stage(&s.empty[st]);
-                    pf_commit(&s.sready[sx]);
-                };
-                for (int x = 0; x < 2 && x < steps && ok; x++) {
-                    if (!pf_wait(&s.qfull[x], nq[x] & 1)) { ok = false; break; }
-                    nq[x]++;
+                const int kind = j.kind, nu = j.u1 - j.u0;
+                if (kind & 4) {              // narrow: not for the tensor core
+                    ahead(st, ph, 2 * nu);
+                    continue;
                 }
-                if (ok) score(0);
+                // A step is 64 keys: both halves of every unit, one after the other, or this stream's half of it. S has two
+                // buffers of 64 columns: the scores of the step after next follow O += P V of this one, so that the softmax
+                // never waits for the tensor core's round trip.
+                const bool two = kind & 2;
+                const int steps = two ? 2 * nu : nu;
+                int ks = st, vs = st;        // next K and V copies
+                uint32_t kp = ph, vp = ph;
+                ahead(vs, vp, 1);
+                auto score = [&](int i) {
+                    const int half = two ? i & 1 : sx;
+                    if (!pf_wait(&s.full[ks], kp)) { ok = false; return; }
+                    pf_fence_after();
+                    pf_mma_qk<D>(tS + (i & 1) * 64, q, ring0 + (uint64_t)(ks * (TB >> 4) + half * (8192 >> 4)), idescS);
+                    pf_commit(&s.sready[sx][i & 1]);
+                    if (!two || half == 1) {
+                        pf_commit_stage(&s.empty[ks]);
+                        ks += 2;
+                        if (ks >= NST) { ks -= NST; kp ^= 1u; }
+                    }
+                };
+                if (!pf_wait(&s.qfull[sx], nq & 1)) { ok = false; break; }
+                nq++;
+                score(0);
                 if (ok && steps > 1) score(1);
                 for (int i = 0; i < steps && ok; i++) {
-                    const int sx = i & 1, unit = pairs ? i >> 1 : i;
-                    const int c = base + pf_stage_v(unit, nu, pairs), st = c % NST;
-                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1)) || !pf_wait(&s.pready[sx], np[sx] & 1)) { ok = false; break; }
+                    const int b = i & 1, half = two ? b : sx;
+                    if (!pf_wait(&s.full[vs], vp) || !pf_wait(&s.pready[sx][b], np[b] & 1)) { ok = false; break; }
+                    np[b]++;
                     pf_fence_after();
-                    const uint32_t v0 = smem_u32(ring + (size_t)st * TB);
-#pragma unroll
-                    for (int kk = 0; kk < kPfKeys / 16; kk++) {
-                        if (kk == kPfKeys / 32) {                     // the second half of P
-                            if (!pf_wait(&s.pready2[sx], np[sx] & 1)) { ok = false; break; }
-                            pf_fence_after();
-                        }
-                        const uint64_t db = pf_desc(v0 + kk * 2048, 16384);
-                        pf_mma_ts(tmem + 256 + sx * 128, tmem + sx * 128 + kk * 8, db, idescO, i >= 2 || kk > 0 ? 1u : 0u);
+                    pf_mma_pv(tO, tS + b * 64, ring0 + kLead + (uint64_t)(vs * (TB >> 4) + half * (8192 >> 4)), idescO, i > 0 ? 1u : 0u);
+                    pf_commit(&s.pvdone[sx]);
+                    if (!two || half == 1) {
+                        pf_commit_stage(&s.empty[vs]);
+                        vs += 2;
+                        if (vs >= NST) { vs -= NST; vp ^= 1u; }
                     }
-                    np[sx]++;
-                    if (!pairs || sx == 1) pf_commit_stage(&s.empty[st]);
-                    if (i + 2 >= steps) pf_commit(&s.odone[sx]);
-                    else score(i + 2);
+                    if (i + 2 < steps) score(i + 2);
                 }
-                base += 2 * nu;
+                ahead(st, ph, 2 * nu);
             }
             if (!ok) s.fail = 1;
         }
@@ -788,11 +869,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         const uint32_t tS = tmem + quarter + sx * 128, tO = tmem + quarter + 256;
         const float sl2 = a.scale * 1.4426950408889634f;
         int base = 0;
-        uint32_t ns = 0, no = 0, nj = 0, nn = 0;
+        uint32_t ns[2] = {0, 0}, n = 0, nj = 0, nn = 0;            // uses of the S buffers, steps, joins, phases of njoin
         uint32_t turn = 0;                                         // narrow jobs seen
         while (pf_next(s, j, nth, ok)) {
-            const int nu = j.u1 - j.u0, tiles = j.tiles(), steps = nu * tiles, keys = j.keys;
-            const bool own = j.own();
+            const int nu = j.u1 - j.u0, keys = j.keys;
+            const bool own = j.own(), two = j.tiles() == 2;
             // what the last jobs left in the streams' Q has been read (pf_narrow looks at its own)
             if (nj > 0 && !pf_wait(&s.join[1], (nj - 1) & 1)) { ok = false; break; }
             if (j.narrow()) {
@@ -802,10 +883,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 continue;
             }
             if (nn > 0 && !pf_wait(&s.njoin[sx], (nn - 1) & 1)) { ok = false; break; }
-            const int mine = (steps + 1 - sx) / 2;                 // steps of this stream
-            if (mine == 0) { base += 2 * nu; continue; }           // (one unit of one tile: the other stream alone)
             // this thread's (row, query head) pair: lane `row` of the tile
-            const int tile0 = (j.grp * 2 + (tiles == 2 ? sx : 0)) * 128, m = tile0 + row;
+            const int tile0 = (j.grp * 2 + (two ? sx : 0)) * 128, m = tile0 + row;
             const int pairsOf = (own ? a.T : a.seqs * a.T) * p.G;
             const bool live = m < pairsOf;
             int see = 0x7FFFFFFF;                                  // keys it sees (a lane without a pair: zeros, never written)
@@ -836,121 +915,47 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             pf_mbar_arrive(&s.qfull[sx]);
 
             float ref = -INFINITY, l = 0.f;                        // reference of the exponents (log2 units), sum
-            // values behind the last key may be anything, and 0 * NaN is NaN: their rows of the stage become zeros
-            auto clear_values = [&](int key0, int unit) {
-                const int kv = keys - key0;
-                if (kv < kPfKeys && (tiles == 1 || sx == 0)) {
-                    const int c = base + pf_stage_v(unit, nu, tiles == 2), st = c % NST;
-                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) return false;
-                    uint8_t* v = ring + (size_t)st * TB;
-                    for (int e = kv * 8 + row; e < kPfKeys * 8; e += 128)
+            const int steps = two ? 2 * nu : nu;
+            for (int i = 0; i < steps; i++) {
+                // this step's 64 keys, in a buffer of their own
+                const int unit = two ? i >> 1 : i, half = two ? i & 1 : sx, b = i & 1, left = keys - (j.u0 + unit) * kPfKeys - half * 64;
+                if (!pf_wait(&s.sready[sx][b], ns[b] & 1)) { ok = false; break; }
+                ns[b]++;
+                pf_fence_after();
+                if (work) {
+                    // (the product before last lies in front of these scores; the last one may still be under way)
+                    auto settled = [&]() {
+                        const bool in = pf_wait(&s.pvdone[sx], (n - 1) & 1);
+                        pf_fence_after();
+                        return in;
+                    };
+                    if (!pf_softmax<T, D>(tS + b * 64, tO + sx * 128, see - keys + left, i == 0, sl2, ref, l, settled)) { ok = false; break; }
+                }
+                if (left < 64) {
+                    // values behind the last key may be anything, and 0 * NaN is NaN: their rows of the stage become zeros
+                    // (of two tiles each stream sees to it for itself, whichever comes first)
+                    const int c = base + 2 * unit + 1, st = c % NST;
+                    if (!pf_wait(&s.full[st], (uint32_t)((c / NST) & 1))) { ok = false; break; }
+                    uint8_t* v = ring + (size_t)st * TB + half * 8192;
+                    for (int e = max(left, 0) * 8 + row; e < 64 * 8; e += 128)
 #pragma unroll
                         for (int x = 0; x < D / 64; x++) *reinterpret_cast<uint4*>(v + x * 16384 + e * 16) = make_uint4(0u, 0u, 0u, 0u);
                     fence_proxy_async_smem();
                 }
-                return true;
-            };
-            for (int i = 0; i < mine && ok; i++) {
-                const int unit = tiles == 2 ? i : 2 * i + sx, key0 = (j.u0 + unit) * kPfKeys;
-                if (!pf_wait(&s.sready[sx], ns & 1)) { ok = false; break; }
-                ns++;
-                pf_fence_after();
-                if (work) {
-                    // scores this row does not see: -infinity, put into tensor memory eight columns at a time (the last
-                    // units of a job only; the code of the common path stays small enough for the instruction caches)
-                    const int nv = see - key0;
-                    if (__any_sync(0xffffffffu, nv < kPfKeys)) {
-                        const int first = max(0, __reduce_min_sync(0xffffffffu, nv)) & ~7;
-#pragma unroll 1
-                        for (int c = first; c < kPfKeys; c += 8) {
-                            uint32_t x[8];
-                            pf_ld8(tS + c, x);
-                            pf_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 8; e++) x[e] = c + e < nv ? x[e] : 0xFF800000u;
-                            pf_st8(tS + c, x);
-                        }
-                        pf_wait_st();
-                    }
-                    uint32_t r[128];
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    pf_ld32(tS, r);
-#pragma unroll
-                    for (int c = 1; c <= 4; c++) {
-                        pf_wait_ld();
-                        if (c < 4) pf_ld32(tS + c * 32, r + c * 32);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) mx[e & 3] = pf_max_nan(mx[e & 3], __uint_as_float(r[(c - 1) * 32 + e]));
-                    }
-                    const float top = pf_max_nan(pf_max_nan(mx[0], mx[1]), pf_max_nan(mx[2], mx[3])) * sl2;
-                    // O and l keep their reference until a score exceeds it by 2^8: then both move to the new maximum
-                    float f = 1.f;
-                    if (!(top <= ref + 8.f) || ref == -INFINITY) {        // (a NaN score makes the whole row NaN)
-                        if (ref != -INFINITY) f = pf_ex2(ref - top);
-                        ref = top;
-                    }
-                    if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-                        l *= f;
-#pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
-                            uint32_t o[16];
-                            pf_ld16(tO + sx * 128 + c, o);
-                            pf_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            pf_st16(tO + sx * 128 + c, o);
-                        }
-                    }
-                    const float off = ref == -INFINITY ? 0.f : -ref;
-                    const uint64_t scale2 = pf_two(sl2, sl2), off2 = pf_two(off, off);
-                    uint64_t sum2[2] = {0, 0};
-                    // P in two halves, so that the tensor core begins with the first while the second is made
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {
-#pragma unroll
-                        for (int c = half * 64; c < half * 64 + 64; c += 2) {
-                            float e0, e1;
-                            const uint64_t x = pf_fma2(pf_two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, off2);
-                            if ((c >> 1) % kPfPolyOf < kPfPoly) {
-                                pf_ex2_poly(x, e0, e1);
-                            } else {
-                                pf_split(x, e0, e1);
-                                e0 = pf_ex2(e0);
-                                e1 = pf_ex2(e1);
-                            }
-                            sum2[(c >> 1) & 1] = pf_add2(sum2[(c >> 1) & 1], pf_two(e0, e1));
-                            r[c >> 1] = pf_pack<T>(e0, e1);
-                        }
-                        pf_st32(tS + half * 32, r + half * 32);
-                        pf_wait_st();
-                        if (half == 0) {
-                            if (!clear_values(key0, unit)) { ok = false; break; }
-                            pf_fence_before();
-                            pf_mbar_arrive(&s.pready[sx]);
-                        }
-                    }
-                    float s0, s1;
-                    pf_split(pf_add2(sum2[0], sum2[1]), s0, s1);
-                    l += s0 + s1;
-                } else {
-                    if (!clear_values(key0, unit)) { ok = false; break; }
-                    pf_mbar_arrive(&s.pready[sx]);
-                }
                 pf_fence_before();
-                pf_mbar_arrive(&s.pready2[sx]);
+                pf_mbar_arrive(&s.pready[sx][b]);
+                n++;
             }
             base += 2 * nu;
             if (!ok) break;
             // ---- the job's partial result
-            if (!pf_wait(&s.odone[sx], no & 1)) { ok = false; break; }
-            no++;
+            if ((steps > 1 && !pf_wait(&s.pvdone[sx], n & 1)) || !pf_wait(&s.pvdone[sx], (n - 1) & 1)) { ok = false; break; }
             pf_fence_after();
-            const bool join = tiles == 1 && steps > 1;           // both streams hold a part of the same tile
-            const int srow = (tiles == 2 ? sx * 128 : 0) + row;
+            const int srow = (two ? sx * 128 : 0) + row;
             const long long at = (long long)j.slot * (own ? p.rowsO : p.rowsP) + srow;
             float2* ml = (own ? p.mlO : p.mlP) + at;
             float* o = (own ? p.oO : p.oP) + at * D;
-            if (!join) {
+            if (two) {
                 if (live) *ml = make_float2(ref, l);
                 if (work) {
 #pragma unroll 1
@@ -965,7 +970,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                     }
                 }
             } else {
-                // the two streams' parts added; each stream's warps write half of the columns
+                // the two streams' parts of the tile added; each stream's warps write half of the columns
                 // (the pairs are exchanged where the streams' Q lay, which no product reads any more)
                 reinterpret_cast<float2*>(smem + sx * TB)[row] = make_float2(ref, l);
                 __syncwarp();
