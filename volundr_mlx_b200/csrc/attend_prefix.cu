@@ -121,7 +121,7 @@ __device__ __forceinline__ int pf_own_keys(const vk_prefix_args& a, int b) {
 __device__ __forceinline__ int pf_nu(int keys) { return (keys + kPfKeys - 1) / kPfKeys; }
 
 struct PfShared {
-    uint64_t full[10], empty[10], qfull[2], sready[2][2], pready[2][2], pvdone[2], join[2], njoin[2], nturn[2], jfull[kPfJobs], jempty[kPfJobs];
+    uint64_t full[10], empty[10], qfull[2], sready[2][2], pready[2][2], pvdone[2][2], join[2], njoin[2], nturn[2], jfull[kPfJobs], jempty[kPfJobs];
     PfJob jobs[kPfJobs];
     int lo, hi, cb0, b0, P, fail;
     uint32_t tmem;
@@ -645,8 +645,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             for (int b = 0; b < 2; b++) {
                 mbar_init(&s.sready[i][b], 1);
                 mbar_init(&s.pready[i][b], 128);
+                mbar_init(&s.pvdone[i][b], 1);
             }
-            mbar_init(&s.pvdone[i], 1);
             mbar_init(&s.join[i], 8);
             mbar_init(&s.njoin[i], 4);
             mbar_init(&s.nturn[i], 4);
@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                     np[b]++;
                     pf_fence_after();
                     pf_mma_pv(tO, tS + b * 64, ring0 + kLead + (uint64_t)(vs * (TB >> 4) + half * (8192 >> 4)), idescO, i > 0 ? 1u : 0u);
-                    pf_commit(&s.pvdone[sx]);
+                    pf_commit(&s.pvdone[sx][b]);
                     if (!two || half == 1) {
                         pf_commit_stage(&s.empty[vs]);
                         vs += 2;
@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         const uint32_t tS = tmem + quarter + sx * 128, tO = tmem + quarter + 256;
         const float sl2 = a.scale * 1.4426950408889634f;
         int base = 0;
-        uint32_t ns[2] = {0, 0}, n = 0, nj = 0, nn = 0;            // uses of the S buffers, steps, joins, phases of njoin
+        uint32_t ns[2] = {0, 0}, nj = 0, nn = 0;                   // uses of the S buffers, joins, phases of njoin
         uint32_t turn = 0;                                         // narrow jobs seen
         while (pf_next(s, j, nth, ok)) {
             const int nu = j.u1 - j.u0, keys = j.keys;
@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 if (work) {
                     // (the product before last lies in front of these scores; the last one may still be under way)
                     auto settled = [&]() {
-                        const bool in = pf_wait(&s.pvdone[sx], (n - 1) & 1);
+                        const bool in = pf_wait(&s.pvdone[sx][b ^ 1], (ns[b ^ 1] - 1) & 1);
                         pf_fence_after();
                         return in;
                     };
@@ -944,12 +944,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 }
                 pf_fence_before();
                 pf_mbar_arrive(&s.pready[sx][b]);
-                n++;
             }
             base += 2 * nu;
             if (!ok) break;
             // ---- the job's partial result
-            if ((steps > 1 && !pf_wait(&s.pvdone[sx], n & 1)) || !pf_wait(&s.pvdone[sx], (n - 1) & 1)) { ok = false; break; }
+            // (a barrier a buffer: at most its last use can still be open, whenever this warp gets here)
+            const int lastb = (steps - 1) & 1;
+            if (!pf_wait(&s.pvdone[sx][lastb], (ns[lastb] - 1) & 1)) { ok = false; break; }
             pf_fence_after();
             const int srow = (two ? sx * 128 : 0) + row;
             const long long at = (long long)j.slot * (own ? p.rowsO : p.rowsP) + srow;
