@@ -192,7 +192,10 @@ __device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t phase) { return 
 __device__ __forceinline__ bool pf_next(PfShared& s, PfJob& j, int& nth, bool& ok) {
     const int q = nth % kPfJobs;
     if (!ok || !pf_wait(&s.jfull[q], (uint32_t)((nth / kPfJobs) & 1))) { ok = false; return false; }
-    j = s.jobs[q];
+    const int* from = reinterpret_cast<const int*>(&s.jobs[q]);
+    int* to = reinterpret_cast<int*>(&j);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(PfJob) / 4); i++) to[i] = __shfl_sync(0xffffffffu, from[i], 0);
     __syncwarp();
     if ((threadIdx.x & 31) == 0) pf_mbar_arrive(&s.jempty[q]);
     nth++;
@@ -636,7 +639,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
     uint8_t* const smem = (uint8_t*)(((uintptr_t)pf_smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* const ring = smem + 2 * TB;
     const vk_prefix_args& a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (warp index, tensor-memory base and jobs are broadcast, so that the compiler knows them to be the same in all lanes and
+    // the MMA warps' operands live in uniform registers)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     if (tid == 0) {
         for (int i = 0; i < NST; i++) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 4); }
@@ -727,7 +732,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
     pf_fence_before();
     __syncthreads();
     pf_fence_after();
-    const uint32_t tmem = s.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem, 0);
     PfJob j;
     bool ok = true;
     int nth = 0;
@@ -811,36 +816,36 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 int ks = st, vs = st;        // next K and V copies
                 uint32_t kp = ph, vp = ph;
                 ahead(vs, vp, 1);
-                auto score = [&](int i) {
-                    const int half = two ? i & 1 : sx;
-                    if (!pf_wait(&s.full[ks], kp)) { ok = false; return; }
-                    pf_fence_after();
-                    pf_mma_qk<D>(tS + (i & 1) * 64, q, ring0 + (uint64_t)(ks * (TB >> 4) + half * (8192 >> 4)), idescS);
-                    pf_commit(&s.sready[sx][i & 1]);
-                    if (!two || half == 1) {
-                        pf_commit_stage(&s.empty[ks]);
-                        ks += 2;
-                        if (ks >= NST) { ks -= NST; kp ^= 1u; }
-                    }
-                };
                 if (!pf_wait(&s.qfull[sx], nq & 1)) { ok = false; break; }
                 nq++;
-                score(0);
-                if (ok && steps > 1) score(1);
-                for (int i = 0; i < steps && ok; i++) {
-                    const int b = i & 1, half = two ? b : sx;
-                    if (!pf_wait(&s.full[vs], vp) || !pf_wait(&s.pready[sx][b], np[b] & 1)) { ok = false; break; }
-                    np[b]++;
-                    pf_fence_after();
-                    pf_mma_pv(tO, tS + b * 64, ring0 + kLead + (uint64_t)(vs * (TB >> 4) + half * (8192 >> 4)), idescO, i > 0 ? 1u : 0u);
-                    pf_commit(&s.pvdone[sx][b]);
-                    if (!two || half == 1) {
-                        pf_commit_stage(&s.empty[vs]);
-                        vs += 2;
-                        if (vs >= NST) { vs -= NST; vp ^= 1u; }
+                for (int k = 0; k < steps + 2; k++) {      // O += P V of step k - 2, then the scores of step k
+                    const int b = k & 1, half = two ? b : sx;
+                    const bool fresh = !two || b == 0, done = !two || b == 1;   // first, last use of a stage by this stream
+                    if (k >= 2) {
+                        if ((fresh && !pf_wait(&s.full[vs], vp)) || !pf_wait(&s.pready[sx][b], np[b] & 1)) { ok = false; break; }
+                        np[b]++;
+                        pf_fence_after();
+                        pf_mma_pv(tO, tS + b * 64, ring0 + kLead + (uint64_t)(vs * (TB >> 4) + half * (8192 >> 4)), idescO, k > 2 ? 1u : 0u);
+                        if (k >= steps) pf_commit(&s.pvdone[sx][b]);       // (before: the next score product's barrier says so)
+                        if (done) {
+                            pf_commit_stage(&s.empty[vs]);
+                            vs += 2;
+                            if (vs >= NST) { vs -= NST; vp ^= 1u; }
+                        }
                     }
-                    if (i + 2 < steps) score(i + 2);
+                    if (k < steps) {
+                        if (fresh && !pf_wait(&s.full[ks], kp)) { ok = false; break; }
+                        pf_fence_after();
+                        pf_mma_qk<D>(tS + b * 64, q, ring0 + (uint64_t)(ks * (TB >> 4) + half * (8192 >> 4)), idescS);
+                        pf_commit(&s.sready[sx][b]);
+                        if (done) {
+                            pf_commit_stage(&s.empty[ks]);
+                            ks += 2;
+                            if (ks >= NST) { ks -= NST; kp ^= 1u; }
+                        }
+                    }
                 }
+                if (!ok) break;
                 ahead(st, ph, 2 * nu);
             }
             if (!ok) s.fail = 1;
@@ -869,7 +874,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
         const uint32_t tS = tmem + quarter + sx * 128, tO = tmem + quarter + 256;
         const float sl2 = a.scale * 1.4426950408889634f;
         int base = 0;
-        uint32_t ns[2] = {0, 0}, nj = 0, nn = 0;                   // uses of the S buffers, joins, phases of njoin
+        uint32_t ns[2] = {0, 0}, nd[2] = {0, 0}, nj = 0, nn = 0;   // uses of the S buffers, phases of pvdone, joins, phases of njoin
         uint32_t turn = 0;                                         // narrow jobs seen
         while (pf_next(s, j, nth, ok)) {
             const int nu = j.u1 - j.u0, keys = j.keys;
@@ -923,9 +928,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
                 ns[b]++;
                 pf_fence_after();
                 if (work) {
-                    // (the product before last lies in front of these scores; the last one may still be under way)
+                    // O += P V of the step before may still be under way when O has to be rescaled. The score product of the
+                    // step after this one is issued behind it; the last two steps have a barrier for it.
                     auto settled = [&]() {
-                        const bool in = pf_wait(&s.pvdone[sx][b ^ 1], (ns[b ^ 1] - 1) & 1);
+                        const bool in = i + 1 < steps ? pf_wait(&s.sready[sx][b ^ 1], ns[b ^ 1] & 1) : pf_wait(&s.pvdone[sx][b ^ 1], nd[b ^ 1] & 1);
                         pf_fence_after();
                         return in;
                     };
@@ -948,9 +954,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             base += 2 * nu;
             if (!ok) break;
             // ---- the job's partial result
-            // (a barrier a buffer: at most its last use can still be open, whenever this warp gets here)
             const int lastb = (steps - 1) & 1;
-            if (!pf_wait(&s.pvdone[sx][lastb], (ns[lastb] - 1) & 1)) { ok = false; break; }
+            if (!pf_wait(&s.pvdone[sx][lastb], nd[lastb] & 1)) { ok = false; break; }
+            nd[lastb]++;
+            if (steps > 1) nd[lastb ^ 1]++;
             pf_fence_after();
             const int srow = (two ? sx * 128 : 0) + row;
             const long long at = (long long)j.slot * (own ? p.rowsO : p.rowsP) + srow;
