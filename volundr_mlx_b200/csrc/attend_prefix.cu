@@ -462,12 +462,13 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
     for (int i = 0; i < 2; i++) {
         const int m = mt * 16 + g + 8 * i, r = (own ? j.b * a.T : 0) + m / p.G;
         const bool live = m < rows;
+        // (a pair beyond the last: some row's queries, no key seen, nothing written)
         const T* q = (const T*)a.q + (live ? r * a.q_row + (j.h * p.G + m % p.G) * a.q_head : 0);
         see[i] = !live ? 0 : own ? min(keys, max(0, a.lens[r])) : keys;
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
-            qa[k][i] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 2 * t) : 0u;
-            qa[k][2 + i] = live ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + 2 * t) : 0u;
+            qa[k][i] = *reinterpret_cast<const uint32_t*>(q + k * 16 + 2 * t);
+            qa[k][2 + i] = *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + 2 * t);
         }
     }
     float o[D / 8][4], ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -908,11 +909,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
 #pragma unroll
                 for (int k = 0; k < 32 / RPI; k++) {
                     const long long at = __shfl_sync(0xffffffffu, qat, k * RPI + lane / LPR);
-                    v[k] = at < 0 ? make_uint4(0u, 0u, 0u, 0u) : reinterpret_cast<const uint4*>((const T*)a.q + at)[c];
+                    v[k] = reinterpret_cast<const uint4*>((const T*)a.q + (at < 0 ? 0 : at))[c];   // (no branch: all loads in flight at once)
                 }
 #pragma unroll
                 for (int k = 0; k < 32 / RPI; k++) {
                     const int qr = (warp & 3) * 32 + k * RPI + lane / LPR;
+                    if (tile0 + qr >= pairsOf) v[k] = make_uint4(0u, 0u, 0u, 0u);
                     *reinterpret_cast<uint4*>(smem + sx * TB + (c >> 3) * 16384 + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v[k];
                 }
             }
