@@ -45,8 +45,6 @@ constexpr int kPfTile = 128, kPfKeys = 128, kPfNarrow = 64;
 // third warpgroup's registers go to the softmax (a row of S is 128 registers): 168 a thread at launch, then 216 + 216 + 72
 constexpr int kPfThreads = 384;
 constexpr int kPfSoftmaxRegs = 216, kPfOtherRegs = 72;
-// Exponentials on the FMA pipe: of every kPfPolyOf pairs of scores the first kPfPoly
-constexpr int kPfPoly = 1, kPfPolyOf = 4;
 constexpr int kPfJobs = 4;               // jobs handed out ahead
 // Lengths on the line of work: a job's fixed part, a unit of one tile, of two tiles, of the narrow form
 struct PfCost { int fixed, one, two; };
@@ -289,23 +287,6 @@ __device__ __forceinline__ float pf_max_nan(float a, float b) {   // NaN if eith
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-// 2^x of two numbers on the FMA pipe, for a part of the exponentials (the special function unit does one warp's worth in
-// eight cycles): x = n + f by rounding, 2^f on [-1/2, 1/2] as the degree-4 polynomial of least relative error (2.7e-6 in fp32,
-// found by exchange iteration), n added to the exponent; zero below 2^-126.
-__device__ __forceinline__ void pf_ex2_poly(uint64_t x, float& e0, float& e1) {
-    const uint64_t r = pf_add2(x, pf_two(12582912.f, 12582912.f));        // 1.5 * 2^23: the integer in the low bits
-    const uint64_t f = pf_fma2(pf_add2(r, pf_two(-12582912.f, -12582912.f)), pf_two(-1.f, -1.f), x);
-    uint64_t q = pf_fma2(pf_two(0.009570102f, 0.009570102f), f, pf_two(0.05591786f, 0.05591786f));
-    q = pf_fma2(q, f, pf_two(0.24024745f, 0.24024745f));
-    q = pf_fma2(q, f, pf_two(0.6931218f, 0.6931218f));
-    q = pf_fma2(q, f, pf_two(0.99999926f, 0.99999926f));
-    float x0, x1, r0, r1, q0, q1;
-    pf_split(x, x0, x1);
-    pf_split(r, r0, r1);
-    pf_split(q, q0, q1);
-    e0 = x0 < -126.f ? 0.f : __uint_as_float(__float_as_uint(q0) + (__float_as_uint(r0) << 23));
-    e1 = x1 < -126.f ? 0.f : __uint_as_float(__float_as_uint(q1) + (__float_as_uint(r1) << 23));
-}
 template <typename T> __device__ __forceinline__ uint32_t pf_pack(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pf_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf2(lo, hi); }
 template <> __device__ __forceinline__ uint32_t pf_pack<__half>(float lo, float hi) {
@@ -422,13 +403,9 @@ __device__ __forceinline__ bool pf_softmax(uint32_t tS, uint32_t tO, int nv, boo
     for (int c = 0; c < N; c += 2) {
         float e0, e1;
         const uint64_t x = pf_fma2(pf_two(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, off2);
-        if ((c >> 1) % kPfPolyOf < kPfPoly) {
-            pf_ex2_poly(x, e0, e1);
-        } else {
-            pf_split(x, e0, e1);
-            e0 = pf_ex2(e0);
-            e1 = pf_ex2(e1);
-        }
+        pf_split(x, e0, e1);
+        e0 = pf_ex2(e0);
+        e1 = pf_ex2(e1);
         sum2[(c >> 1) & 1] = pf_add2(sum2[(c >> 1) & 1], pf_two(e0, e1));
         r[c >> 1] = pf_pack<T>(e0, e1);
     }
