@@ -135,6 +135,19 @@ def test_sharp_and_flat_scores(cuda):
     c.check()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,KVH", [(40, 2), (2, 2)])
+def test_one_key_far_above_many(cuda, dtype, H, KVH):
+    """One key of the prefix takes as much as thousands of small ones together: their probabilities are 2^-14 and less of the
+    largest, where fp16 without a common factor has lost most of its bits."""
+    c = Case(H, KVH, 64, 9000, [1000, 5, 0, 64], seed=22, dtype=dtype, spread=0.0)
+    c.q.fill_(0.5)
+    fin = torch.isfinite(c.K)
+    c.K.copy_(torch.where(fin, torch.zeros_like(c.K), c.K))
+    c.K[int(c.prefix_pages[3]), :, 17] = 2.5            # score 64 * 0.5 * 2.5 / 8 = 10: e^-10 = 4.5e-5 = 2^-14.4
+    c.check()
+
+
 def test_long_prefix_and_long_own(cuda):
     Case(10, 2, 128, 20011, [1, 4000, 17], seed=11).check()
     Case(16, 16, 64, 130, [9000, 3, 12345], seed=12).check()

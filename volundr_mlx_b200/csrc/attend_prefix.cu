@@ -29,7 +29,7 @@ extern "C" struct vk_prefix_args {
 namespace {
 
 // A unit of work is 128 keys of one kv head against a tile of (row, query head) pairs. Two forms:
-//   wide   up to 128 pairs, one tensor-memory lane each: S[128 x 128] = Q K^T (tcgen05.mma, Q and K in shared memory),
+//   wide   up to 128 pairs, one tensor-memory lane each: S[128 x 64] = Q K^T (tcgen05.mma, Q and K in shared memory),
 //          P = exp2(S - m) in registers, O[128 x D] += P V with P in tensor memory (over S) and V in shared memory. Two
 //          streams (a softmax warpgroup and a warp that issues its MMAs each) share the tensor core: two tiles on the same keys,
 //          or one tile on the two 64-key halves of every unit;
@@ -40,11 +40,19 @@ namespace {
 // A job is a run of units: a tile, or two tiles that share the keys, against the prefix or against one sequence's own keys.
 // All jobs lie on one line, each as long as it is expected to take, and every CTA takes an equal interval of it.
 constexpr int kPfTile = 128, kPfKeys = 128, kPfNarrow = 64;
-// warps 0-3 and 4-7: softmax of two streams; 8: copies; 9, 11: MMAs of the streams (one warp for both took 4400 cycles for what the
-// tensor core does in 2050: its own instructions were the limit); 10: walks the line of work and hands out the jobs. The
-// third warpgroup's registers go to the softmax (a row of S is 128 registers): 168 a thread at launch, then 216 + 216 + 72
+// Measured (128 rows x 40 heads of 128 behind 32768 keys, 2 to 1024 own): 140 us, 52 at the tensor core's rate; prefix alone 111,
+// own keys alone 43 (131 MB). The prefix takes 2600 cycles per 64 keys of two tiles where its MMAs take 1330 and its softmax
+// 1300 a stream: what bounds it is the chain of a stream (scores -> softmax -> P -> next scores), which two S buffers do not
+// cover. With S in one buffer of 128 keys a stream the same took 152 us. 16 rows behind 20000 keys: 45 us, 20 at HBM's
+// rate; about 13 us of it are the start (lengths, the line, the first job, its queries and keys: one round trip after
+// another) and 5 the merge.
+// warps 0-3 and 4-7: softmax of two streams; 8: copies; 9, 11: MMAs of the streams; 10: walks the line of work and hands out the
+// jobs. The third warpgroup's registers go to the softmax and the narrow form: 168 a thread at launch, then 216 + 216 + 72
 constexpr int kPfThreads = 384;
 constexpr int kPfSoftmaxRegs = 216, kPfOtherRegs = 72;
+// Probabilities meet the values in the storage type. They are at most 2^8 (below); as fp16 they are raised by 2^7, which keeps
+// those down to 2^-21 of the largest above fp16's subnormal numbers (bf16 has fp32's range).
+template <typename T> constexpr float kPfRaise = std::is_same<T, __half>::value ? 7.f : 0.f;
 constexpr int kPfJobs = 4;               // jobs handed out ahead
 // Lengths on the line of work: a job's fixed part, a unit of one tile, of two tiles, of the narrow form
 struct PfCost { int fixed, one, two; };
@@ -396,7 +404,7 @@ __device__ __forceinline__ bool pf_softmax(uint32_t tS, uint32_t tO, int nv, boo
             pf_st16(tO + c, o);
         }
     }
-    const float off = ref == -INFINITY ? 0.f : -ref;
+    const float off = ref == -INFINITY ? 0.f : kPfRaise<T> - ref;
     const uint64_t scale2 = pf_two(sl2, sl2), off2 = pf_two(off, off);
     uint64_t sum2[2] = {0, 0};
 #pragma unroll
@@ -501,7 +509,7 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
 #pragma unroll
                         for (int n = 0; n < D / 8; n++) { o[n][2 * i] *= f; o[n][2 * i + 1] *= f; }
                     }
-                    const float off = ref[i] == -INFINITY ? 0.f : ref[i];
+                    const float off = ref[i] == -INFINITY ? 0.f : ref[i] - kPfRaise<T>;
 #pragma unroll
                     for (int n = 0; n < 4; n++)
 #pragma unroll
@@ -555,7 +563,7 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
         for (int i = 0; i < 2; i++) {
             const int m = mt * 16 + g + 8 * i;
             if (m < rows) {
-                if (t == 0) ml[m] = make_float2(ref[i], l[i]);
+                if (t == 0) ml[m] = make_float2(ref[i] - kPfRaise<T>, l[i]);
 #pragma unroll
                 for (int n = 0; n < D / 8; n++) *reinterpret_cast<float2*>(out + m * D + n * 8 + 2 * t) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
             }
@@ -568,7 +576,7 @@ __device__ __forceinline__ bool pf_narrow(const PfParams& p, PfShared& s, const 
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         const int row = g + 8 * i;
-        if (t == 0) s.ml[sx * 4 + warp][row] = make_float2(ref[i], l[i]);
+        if (t == 0) s.ml[sx * 4 + warp][row] = make_float2(ref[i] - kPfRaise<T>, l[i]);
 #pragma unroll
         for (int n = 0; n < D / 8; n++)   // (blocks of eight columns swapped by row: the eight rows of a store hit different banks)
             *reinterpret_cast<float2*>(buf + (warp * 16 + row) * D + ((n ^ (row & 7)) * 8 + 2 * t)) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
@@ -943,7 +951,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             float2* ml = (own ? p.mlO : p.mlP) + at;
             float* o = (own ? p.oO : p.oP) + at * D;
             if (two) {
-                if (live) *ml = make_float2(ref, l);
+                if (live) *ml = make_float2(ref - kPfRaise<T>, l);
                 if (work) {
 #pragma unroll 1
                     for (int c = 0; c < D / 32; c++) {
@@ -959,7 +967,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             } else {
                 // the two streams' parts of the tile added; each stream's warps write half of the columns
                 // (the pairs are exchanged where the streams' Q lay, which no product reads any more)
-                reinterpret_cast<float2*>(smem + sx * TB)[row] = make_float2(ref, l);
+                reinterpret_cast<float2*>(smem + sx * TB)[row] = make_float2(ref - kPfRaise<T>, l);
                 __syncwarp();
                 if (lane == 0) pf_mbar_arrive(&s.join[0]);
                 if (!pf_wait(&s.join[0], nj & 1)) { ok = false; break; }
@@ -1134,7 +1142,8 @@ template <typename T, int D> cudaError_t pf_launch(const PfParams& p, int sms, c
     // fit the instruction cache that the SMs share).
     e = vk_launch_cluster(attend_prefix_kernel<T, D>, dim3((unsigned)sms), dim3(kPfThreads), 2, PfCfg<D>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
-    // (a warp a pair from about four warps an SM on: attend of 16 rows x 40 heads takes MERGE_A us, MERGE_B with split pieces)
+    // (eight warps a pair while that gives each SM no more than a few CTAs: 640 pairs of 18 pieces took 13 us longer with a
+    // warp each; 5120 pairs of 7 pieces take 8 us with a warp each and 23 with four)
     const int pairs = p.a.seqs * p.a.T * p.a.Hq;
     if (pairs <= 8 * sms) return vk_launch(attend_prefix_merge_kernel<T, D, true>, dim3((unsigned)pairs), dim3(256), 0, stream, p);
     return vk_launch(attend_prefix_merge_kernel<T, D, false>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p);
@@ -1188,6 +1197,7 @@ size_t pf_layout(PfParams& p, const vk_prefix_args* a, uint8_t* ws, int ctas) {
     p.ST = (int)((mO + 127) / 128);
     p.narrowP = mP <= kPfNarrow;
     p.narrowO = mO <= kPfNarrow;
+    // (lengths fitted to the times of the CTAs; 1 : 1.2 between the forms, or a fixed part of 6 to 16, changed the cases by 3% and less)
     p.costP = p.costO = PfCost{4, 4, 8};
     p.longest = max(p.MT > 1 ? p.costP.two : p.costP.one, p.ST > 1 ? p.costO.two : p.costO.one);
     p.rowsP = (int)(mP < 256 ? mP : 256);
