@@ -351,7 +351,9 @@ int vk_kv_append(const vk_append_args* a, vk_stream_t stream);
  * 16-byte aligned, strides multiples of 8. lens[r] < 0: a padded row, its output is left as it was; no visible key:
  * zeros. Lengths beyond the page lists are clamped, pages outside the pool replaced by page 0, both reported in the status
  * word. At most 65536 rows and 2^31 - 1 key rows (n_pages * KVH * 64) in the pool, else -3. The per-sequence form is
- * vk_attend_decode. workspace: scratch of the call, needs no initial value; calls that overlap on the GPU need one each. */
+ * vk_attend_decode. workspace: scratch of the call, needs no initial value; calls that overlap on the GPU need one each. The
+ * first call on each device outside stream capture (shared-memory opt-in). What a row does not see may hold anything, except
+ * that the values one of a sequence's T rows sees must be finite for all of them (a weight of zero times infinity). */
 typedef struct vk_prefix_args {
     int dtype, seqs, T, Hq, KVH, D;
     float scale;

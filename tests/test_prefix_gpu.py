@@ -274,3 +274,34 @@ def test_steps_of_rotate_append_attend(cuda):
         ops.check_status()
         check_attend(out, attend(q, K, V, prefix, P, table, lens, 1), before)
         slot = torch.where(live, slot + 1, slot)
+
+
+def test_wrappers_refuse(cuda):
+    """Wrong shapes, types, strides and gradients never reach a launch."""
+    from volundr_mlx_b200 import ops, rotary
+
+    c = Case(4, 2, 64, 100, [30, 40], seed=23)
+    a = dict(q=c.q, K=c.K, V=c.V, prefix_pages=c.prefix_pages, prefix_len=c.prefix_len, table=c.table, lens=c.lens)
+    ops.attend_prefix(**a)
+    wide = torch.zeros((2, 4, 72), device="cuda", dtype=c.q.dtype)
+    for bad in (dict(q=c.q.float()), dict(q=c.q.half()), dict(q=c.q[:, :3]), dict(q=wide[:, :, 4:68]), dict(K=c.K.transpose(0, 1)),
+                dict(V=c.V[:, :1]), dict(lens=c.lens[:1]), dict(lens=c.lens.long()), dict(prefix_len=c.prefix_len.long()),
+                dict(prefix_pages=c.prefix_pages[None]), dict(table=c.table[:1]), dict(table=c.table.cpu()), dict(T=0), dict(T=2),
+                dict(scale=0.0), dict(scale=-1.0), dict(gate=c.q[:1]), dict(out=c.q[:, :, :32]),
+                dict(q=c.q.clone().requires_grad_(True))):
+        with pytest.raises(ValueError):
+            ops.attend_prefix(**{**a, **bad})
+    freq, _ = rotary.frequencies(64, 1e4, device="cuda")
+    pos = torch.zeros(2, device="cuda", dtype=torch.int32)
+    k = torch.zeros((2, 2, 64), device="cuda", dtype=c.q.dtype)
+    for bad in (dict(pos=pos.long()), dict(freq=freq.float()), dict(freq=torch.ones(33, device="cuda", dtype=torch.float64)),
+                dict(out=torch.zeros((2, 2, 32), device="cuda", dtype=c.q.dtype)), dict(x=k.float()), dict(x=k.transpose(1, 2)),
+                dict(out=k.transpose(0, 1))):
+        with pytest.raises(ValueError):
+            ops.rope(**{**dict(x=k, pos=pos, freq=freq), **bad})
+    b = dict(k=k, v=k, K=c.K, V=c.V, table=c.table, pos=pos, freq=freq)
+    for bad in (dict(v=k[:1]), dict(v=k.half()), dict(K=c.K[:, :1]), dict(table=c.table[0]), dict(slot=pos[:1]), dict(seq=pos.long()),
+                dict(q=c.q[:1]), dict(q_out=c.q), dict(table=c.table[:1])):
+        with pytest.raises(ValueError):
+            ops.kv_append(**{**b, **bad})
+    ops.check_status()

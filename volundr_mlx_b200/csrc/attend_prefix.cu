@@ -39,7 +39,7 @@ namespace {
 //          between warps and tensor core, and a 16-row tile does not pay for 128.
 // A job is a run of units: a tile, or two tiles that share the keys, against the prefix or against one sequence's own keys.
 // All jobs lie on one line, each as long as it is expected to take, and every CTA takes an equal interval of it.
-constexpr int kPfTile = 128, kPfKeys = 128, kPfNarrow = 64;
+constexpr int kPfKeys = 128, kPfNarrow = 64;   // (with the wide form for everything four of the cases took 80 / 120 / 91 / 557 us, with both 54 / 56 / 63 / 196)
 // Measured (128 rows x 40 heads of 128 behind 32768 keys, 2 to 1024 own): 140 us, 52 at the tensor core's rate; prefix alone 111,
 // own keys alone 43 (131 MB). The prefix takes 2600 cycles per 64 keys of two tiles where its MMAs take 1330 and its softmax
 // 1300 a stream: what bounds it is the chain of a stream (scores -> softmax -> P -> next scores), which two S buffers do not
@@ -121,7 +121,13 @@ __device__ __forceinline__ int pf_clamp(int n, int pages) {
 // Keys of sequence b's own pages that any of its rows sees
 __device__ __forceinline__ int pf_own_keys(const vk_prefix_args& a, int b) {
     int n = 0;
-    for (int t = 0; t < a.T; t++) n = max(n, a.lens[b * a.T + t]);
+    for (int t = 0; t < a.T; t += 8) {      // (eight loads at once: one after another a window of eight tokens took 3 us)
+        int v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] = t + u < a.T ? a.lens[b * a.T + t + u] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; u++) n = max(n, v[u]);
+    }
     return pf_clamp(n, a.max_pages);
 }
 __device__ __forceinline__ int pf_nu(int keys) { return (keys + kPfKeys - 1) / kPfKeys; }
@@ -283,11 +289,6 @@ __device__ __forceinline__ uint64_t pf_fma2(uint64_t a, uint64_t b, uint64_t c) 
 __device__ __forceinline__ uint64_t pf_add2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t pf_mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 __device__ __forceinline__ float pf_max_nan(float a, float b) {   // NaN if either is
