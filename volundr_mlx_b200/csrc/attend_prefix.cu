@@ -739,8 +739,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) attend_prefix_kernel(const __gr
             for (int c = 0; c < 2 * nu && ok; c++) {
                 const int i = c >> 1, isv = c & 1;
                 const int st = n % NST;
-                // (the first job's Q is read before the ring's first load fills the memory system: behind it, it took up to 7 us)
-                if (n == 2 && nth == 1 && !j.narrow() && !pf_wait(&s.qfull[0], 0)) { ok = false; break; }
                 if (n >= NST && !pf_wait(&s.empty[st], (uint32_t)((n / NST - 1) & 1))) { ok = false; break; }
                 const int pg = (j.u0 + i) * 2, cnt = min(2, pages - pg);
                 if (pg - ids0 >= 32) {
@@ -1138,10 +1136,7 @@ template <typename T, int D> cudaError_t pf_launch(const PfParams& p, int sms, c
     static PerDeviceOnce once;
     cudaError_t e = once.run([] { return cudaFuncSetAttribute(attend_prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PfCfg<D>::kSmem); });
     if (e != cudaSuccess) return e;
-    // Pairs of neighbours on the line of work as clusters, so that both SMs of a TPC run the same form: a CTA of the wide form
-    // beside one of the narrow form ran its softmax 1.1 to 1.25 times as long and its steps 1.4 times (the two loops do not
-    // fit the instruction cache that the SMs share).
-    e = vk_launch_cluster(attend_prefix_kernel<T, D>, dim3((unsigned)sms), dim3(kPfThreads), 2, PfCfg<D>::kSmem, stream, p);
+    e = vk_launch(attend_prefix_kernel<T, D>, dim3((unsigned)sms), dim3(kPfThreads), PfCfg<D>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
     // (eight warps a pair while that gives each SM no more than a few CTAs: 640 pairs of 18 pieces took 13 us longer with a
     // warp each; 5120 pairs of 7 pieces take 8 us with a warp each and 23 with four)
@@ -1172,7 +1167,7 @@ int prefix_args_ok(const vk_prefix_args* a) {
     return VK_OK;
 }
 
-// One CTA per SM (148, the target's count, where no device answers), an even number.
+// One CTA per SM (148, the target's count, where no device answers).
 int pf_ctas() {
     static std::atomic<int> sms{0};
     int n = sms.load(std::memory_order_acquire);
@@ -1182,7 +1177,6 @@ int pf_ctas() {
             cudaGetLastError();
             return 148;
         }
-        n = n < 2 ? 2 : n & ~1;
         sms.store(n, std::memory_order_release);
     }
     return n;
