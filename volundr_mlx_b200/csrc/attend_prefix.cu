@@ -40,7 +40,7 @@ namespace {
 // A job is a run of units: a tile, or two tiles that share the keys, against the prefix or against one sequence's own keys.
 // All jobs lie on one line, each as long as it is expected to take, and every CTA takes an equal interval of it.
 constexpr int kPfKeys = 128, kPfNarrow = 64;   // (with the wide form for everything four of the cases took 80 / 120 / 91 / 557 us, with both 54 / 56 / 63 / 196)
-// Measured (128 rows x 40 heads of 128 behind 32768 keys, 2 to 1024 own): 140 us, 52 at the tensor core's rate; prefix alone 111,
+// Measured (128 rows x 40 heads of 128 behind 32768 keys, 16 to 1024 own): 137 us, 52 at the tensor core's rate; prefix alone 111,
 // own keys alone 43 (131 MB). The prefix takes 2600 cycles per 64 keys of two tiles where its MMAs take 1330 and its softmax
 // 1300 a stream: what bounds it is the chain of a stream (scores -> softmax -> P -> next scores), which two S buffers do not
 // cover. With S in one buffer of 128 keys a stream the same took 152 us. 16 rows behind 20000 keys: 45 us, 20 at HBM's
@@ -372,13 +372,12 @@ __device__ __forceinline__ bool pf_softmax(uint32_t tS, uint32_t tO, int nv, boo
     uint32_t r[N];
     float mx[8];
     pf_ld32(tS, r);
-    pf_wait_ld();
     pf_ld32(tS + 32, r + 32);
+    pf_wait_ld();
 #pragma unroll
     for (int e = 0; e < 8; e++) mx[e] = __uint_as_float(r[e]);
 #pragma unroll
     for (int e = 8; e < 32; e++) mx[e & 7] = pf_max_nan(mx[e & 7], __uint_as_float(r[e]));
-    pf_wait_ld();
 #pragma unroll
     for (int e = 32; e < 64; e++) mx[e & 7] = pf_max_nan(mx[e & 7], __uint_as_float(r[e]));
 #pragma unroll
