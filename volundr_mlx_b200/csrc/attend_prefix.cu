@@ -1138,7 +1138,7 @@ template <typename T, int D> cudaError_t pf_launch(const PfParams& p, int sms, c
     e = vk_launch(attend_prefix_kernel<T, D>, dim3((unsigned)sms), dim3(kPfThreads), PfCfg<D>::kSmem, stream, p);
     if (e != cudaSuccess) return e;
     // (eight warps a pair while that gives each SM no more than a few CTAs: 640 pairs of 18 pieces took 13 us longer with a
-    // warp each; 5120 pairs of 7 pieces take 8 us with a warp each and 23 with four)
+    // warp each; 5120 pairs of 7 pieces take 13 us with a warp each and 23 with four, caches cold)
     const int pairs = p.a.seqs * p.a.T * p.a.Hq;
     if (pairs <= 8 * sms) return vk_launch(attend_prefix_merge_kernel<T, D, true>, dim3((unsigned)pairs), dim3(256), 0, stream, p);
     return vk_launch(attend_prefix_merge_kernel<T, D, false>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p);

@@ -148,6 +148,8 @@ template <typename T> cudaError_t rope_launch(int vec, const RopeParams& p, int 
 }
 
 // The widest piece every pointer and stride allows: 16 bytes, 4 bytes or one element.
+// (16384 rows of 40 heads of 128, interleaved: 77 us with 16 bytes, 175 with 4, 173 with one element; the append of 16380 rows in
+// the half layout 87, 148, 247)
 struct PieceRule {
     uintptr_t bits = 0;
     void rows(const void* p, long long row, long long head) { bits |= (uintptr_t)p | (uintptr_t)(row * 2) | (uintptr_t)(head * 2); }
