@@ -168,6 +168,14 @@ def test_many_jobs_a_processor(cuda, D, T):
     Case(390, 3, D, 130, lens[: 20 * T], T=T, seed=20).check()
 
 
+@pytest.mark.parametrize("S", [385, 1000])
+def test_more_sequences_than_threads(cuda, S):
+    """The lengths are summed in several rounds; most sequences are empty or padding, some far between are not."""
+    Case(2, 1, 64, 100, [(7 * i) % 130 for i in range(S)], seed=24).check()
+    Case(6, 2, 128, 65, [300 if i % 97 == 5 else (0 if i % 2 else -1) for i in range(S)], seed=25, gate=True).check()
+    Case(2, 1, 64, 0, [200 if i >= S - 2 else 0 for i in range(S)], seed=26, dtype=torch.float16).check()
+
+
 def test_same_bits_every_time(cuda):
     c = Case(40, 8, 128, 3000, [5, 900, 64, 65, 1, 0, 2000], seed=14)
     a = c.run().clone()
